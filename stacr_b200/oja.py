@@ -14,8 +14,12 @@ import torch
 
 
 def orthonormalize(matrix: torch.Tensor) -> torch.Tensor:
-    """Orthonormal basis of the column span, computed in fp32 and returned in the input dtype."""
-    q = torch.linalg.qr(matrix.float(), mode="reduced").Q
+    """Orthonormal basis of the column span, computed in fp32 and returned in the input dtype.
+
+    Row-major, as a basis restored from a state dict is: the factorisation returns its columns contiguous, and products
+    with the two layouts may round differently, so that a resumed layer would leave the trajectory of the saved one.
+    """
+    q = torch.linalg.qr(matrix.float(), mode="reduced").Q.contiguous()
     return q.to(matrix.dtype)
 
 
