@@ -24,6 +24,7 @@ from torch import nn
 import stacr_b200 as S
 from stacr_b200.adaptive import STACRConfig as AdaptiveConfig, STACRLinear as AdaptiveLinear, get_basis_pool, set_stacr_runtime_state
 from stacr_b200.models import build_model
+from stacr_b200.optim import clip_grad_norm_
 from stacr_b200.parallel import GradSync, broadcast_parameters
 from stacr_b200.protocols.baselines.amp import AMPManager
 from stacr_b200.protocols.baselines.checkpointing import apply_checkpointing
@@ -777,7 +778,7 @@ def run_convergence_experiment(cfg: ConvergenceConfig, logger) -> Dict[str, Any]
                         sync_replicated_grads(model, None)
                     if cfg.grad_clip > 0:
                         amp.unscale_(optimizer)
-                        torch.nn.utils.clip_grad_norm_(model.parameters(), cfg.grad_clip)
+                        clip_grad_norm_(model.parameters(), cfg.grad_clip)
                     amp.step(optimizer)
             loss_sum += value
             tokens += int(batch["attention_mask"].sum())

@@ -21,6 +21,7 @@ import torch.distributed as dist
 from torch import nn
 
 from stacr_b200 import memory_accounting as acct
+from stacr_b200.optim import clip_grad_norm_
 from stacr_b200.protocols.profiling import read_peaks
 
 __all__ = [
@@ -377,7 +378,7 @@ def train_epoch(model: nn.Module, train_loader, criterion, optimizer, scheduler,
             if grad_clip and grad_clip > 0:
                 if amp_manager is not None:
                     amp_manager.unscale_(optimizer)
-                torch.nn.utils.clip_grad_norm_(model.parameters(), grad_clip)
+                clip_grad_norm_(model.parameters(), grad_clip)
             amp_manager.step(optimizer) if amp_manager is not None else optimizer.step()
             if scheduler is not None:
                 scheduler.step()

@@ -46,6 +46,13 @@ class Linear(nn.Linear):
         return nn_ops.linear(x, self.weight, self.bias)
 
 
+def is_plain_linear(module: nn.Module) -> bool:
+    """Whether calling ``module`` computes ``nn_ops.linear`` of its weight and bias and nothing else, so that its operands may be used
+    directly: not a wrapped, compressed, adapted or hooked layer."""
+    return (type(module) is Linear and "forward" not in module.__dict__ and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
 class Embedding(nn.Embedding):
     """``nn.Embedding`` (same parameter, same state-dict key) whose bf16-autocast path on a B200 is the in-tree lookup and
     scatter-add (see ``ops.nn_ops.embedding``); the output is then already in the autocast dtype."""

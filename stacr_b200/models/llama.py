@@ -3,12 +3,13 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 from torch import nn
-from torch.nn import functional as F
 
-from .common import causal_attention, Embedding, init_weights, Linear, lm_loss, ModelOutput
+from ..ops import nn_ops
+from .common import causal_attention, Embedding, init_weights, is_plain_linear, Linear, lm_loss, ModelOutput
 from .neox import apply_rotary, rotary_tables
 
 
@@ -26,6 +27,8 @@ class LlamaConfig:
     attention_bias: bool = False
     tie_word_embeddings: bool = False
     loss_chunk: int = 0
+    rope_scaling: Optional[dict] = None     # see ``ops.nn_ops.rotary_frequencies``
+    mlp_recompute: bool = False             # form the MLP's two projections again in backward instead of keeping them
 
 
 PRESETS = {
@@ -55,23 +58,36 @@ class LlamaAttention(nn.Module):
         super().__init__()
         self.n_head, self.n_kv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.head_dim = cfg.hidden_size // cfg.num_attention_heads
-        self.theta = cfg.rope_theta
+        self.theta, self.scaling = cfg.rope_theta, cfg.rope_scaling
         self.q_proj = Linear(cfg.hidden_size, self.n_head * self.head_dim, bias=cfg.attention_bias)
         self.k_proj = Linear(cfg.hidden_size, self.n_kv * self.head_dim, bias=cfg.attention_bias)
         self.v_proj = Linear(cfg.hidden_size, self.n_kv * self.head_dim, bias=cfg.attention_bias)
         self.o_proj = Linear(self.n_head * self.head_dim, cfg.hidden_size, bias=False)
         self._tables = None
+        self._frequencies = None
+
+    def _rotate(self, q, k):
+        s, device = q.shape[1], q.device
+        if device.type == "cuda" or self.scaling:
+            key = (s if self.scaling else None, device)      # a dynamic scaling depends on the length
+            if self._frequencies is None or self._frequencies[0] != key:
+                self._frequencies = (key, nn_ops.rotary_frequencies(self.head_dim, self.theta, self.scaling, seq_len=s, device=device))
+            inv, scale = self._frequencies[1]
+            q, k = nn_ops.rotary(q, k, inv, scale=scale)
+            return q.transpose(1, 2), k.transpose(1, 2)
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+        key = (s, device, q.dtype)
+        if self._tables is None or self._tables[0] != key:
+            self._tables = (key, rotary_tables(s, self.head_dim, self.theta, device, q.dtype))
+        cos, sin = self._tables[1]
+        return apply_rotary(q, cos, sin, self.head_dim), apply_rotary(k, cos, sin, self.head_dim)
 
     def forward(self, x, attention_mask=None):
         b, s, _ = x.shape
-        q = self.q_proj(x).view(b, s, self.n_head, self.head_dim).transpose(1, 2)
-        k = self.k_proj(x).view(b, s, self.n_kv, self.head_dim).transpose(1, 2)
+        q = self.q_proj(x).view(b, s, self.n_head, self.head_dim)
+        k = self.k_proj(x).view(b, s, self.n_kv, self.head_dim)
         v = self.v_proj(x).view(b, s, self.n_kv, self.head_dim).transpose(1, 2)
-        key = (s, x.device, q.dtype)
-        if self._tables is None or self._tables[0] != key:
-            self._tables = (key, rotary_tables(s, self.head_dim, self.theta, x.device, q.dtype))
-        cos, sin = self._tables[1]
-        q, k = apply_rotary(q, cos, sin, self.head_dim), apply_rotary(k, cos, sin, self.head_dim)
+        q, k = self._rotate(q, k)
         if self.n_kv != self.n_head:
             rep = self.n_head // self.n_kv
             k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
@@ -85,9 +101,15 @@ class LlamaMLP(nn.Module):
         self.gate_proj = Linear(cfg.hidden_size, cfg.intermediate_size, bias=False)
         self.up_proj = Linear(cfg.hidden_size, cfg.intermediate_size, bias=False)
         self.down_proj = Linear(cfg.intermediate_size, cfg.hidden_size, bias=False)
+        self.recompute = cfg.mlp_recompute
 
     def forward(self, x):
-        return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+        gate, up = self.gate_proj, self.up_proj
+        if is_plain_linear(gate) and is_plain_linear(up) and nn_ops.gated_linear_supported(x, gate.weight, up.weight):
+            h = nn_ops.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, recompute=self.recompute)
+        else:                       # compressed or adapted projections, other devices and types
+            h = nn_ops.gated_product(gate(x), up(x))
+        return self.down_proj(h)
 
 
 class LlamaDecoderLayer(nn.Module):

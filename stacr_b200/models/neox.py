@@ -72,6 +72,7 @@ class NeoXAttention(nn.Module):
         self.attention_dropout = cfg.attention_dropout
         self._tables = None
         self._half = None
+        self._inv_freq = None
 
     def _rotary(self, seq, device, dtype):
         key = (seq, device, dtype)
@@ -104,9 +105,16 @@ class NeoXAttention(nn.Module):
             q, k, v = (t.transpose(1, 2) for t in qkv.view(b, s, self.n_head, 3 * self.head_dim).split(self.head_dim, dim=-1))
         else:
             # NeoX interleaves per head: [H, 3 * head_dim]
-            q, k, v = (t.transpose(1, 2) for t in qkv.view(b, s, self.n_head, 3 * self.head_dim).split(self.head_dim, dim=-1))
-            cos, sin = self._rotary(s, x.device, q.dtype)
-            q, k = apply_rotary(q, cos, sin, self.rot), apply_rotary(k, cos, sin, self.rot)
+            q, k, v = qkv.view(b, s, self.n_head, 3 * self.head_dim).split(self.head_dim, dim=-1)
+            if x.is_cuda and self.rot and self.rot % 2 == 0:
+                if self._inv_freq is None or self._inv_freq.device != x.device:
+                    self._inv_freq = nn_ops.rotary_frequencies(self.rot, self.base, device=x.device)[0]
+                q, k = nn_ops.rotary(q, k, self._inv_freq)
+                q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+            else:
+                q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+                cos, sin = self._rotary(s, x.device, q.dtype)
+                q, k = apply_rotary(q, cos, sin, self.rot), apply_rotary(k, cos, sin, self.rot)
         ctx = causal_attention(q, k, v, causal=True, attention_mask=attention_mask, dropout_p=self.attention_dropout, training=self.training)
         return self.dense(ctx.transpose(1, 2).reshape(b, s, d))
 

@@ -9,6 +9,7 @@ False.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -186,6 +187,11 @@ def sm_count(device=None) -> int:
     if idx not in _sms:
         _sms[idx] = torch.cuda.get_device_properties(idx).multi_processor_count
     return max(1, _sms[idx] - _reserved_sms)
+
+
+def on_device(t: torch.Tensor):
+    """Context in which the current device, and with it the stream that :func:`stream_ptr` returns, is the tensor's."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

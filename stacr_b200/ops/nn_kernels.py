@@ -1,4 +1,4 @@
-"""ctypes entry points for ``csrc/nn_kernels.cu`` (LayerNorm, GELU, cross-entropy, casts)."""
+"""ctypes entry points for ``csrc/nn_kernels.cu`` (LayerNorm, GELU, cross-entropy, casts), ``csrc/gated.cu`` and ``csrc/rotary.cu``."""
 
 from __future__ import annotations
 
@@ -175,3 +175,53 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, vocab: int, padding_idx: 
     _lib.check_rc(rc, "sb_embedding_bwd")
     _lib.count(1)
     return out
+
+
+DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+ACTIVATION_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def gated_product_fwd(gate: torch.Tensor, up: torch.Tensor, activation: str) -> torch.Tensor:
+    """``act(gate) * up`` of two ``[rows, n]`` matrices with contiguous columns; the result is contiguous."""
+    rows, n = gate.shape
+    out = torch.empty(rows, n, dtype=gate.dtype, device=gate.device)
+    rc = _lib.load().sb_gated_product_fwd(_lib.ptr(gate), _lib.ptr(up), _lib.ptr(out), c_ll(gate.stride(0)), c_ll(up.stride(0)), c_ll(rows), c_ll(n),
+                                          c_int(DTYPE_CODE[gate.dtype]), c_int(ACTIVATION_CODE[activation]), c_int(_lib.sm_count(gate.device)),
+                                          _lib.stream_ptr())
+    _lib.check_rc(rc, "sb_gated_product_fwd")
+    _lib.count(1)
+    return out
+
+
+def gated_product_bwd(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activation: str, need_gate: bool = True, need_up: bool = True):
+    """``(dgate, dup)`` of :func:`gated_product_fwd`, contiguous; ``None`` for one that is not needed."""
+    rows, n = gate.shape
+    dgate = torch.empty(rows, n, dtype=gate.dtype, device=gate.device) if need_gate else None
+    dup = torch.empty(rows, n, dtype=gate.dtype, device=gate.device) if need_up else None
+    rc = _lib.load().sb_gated_product_bwd(_lib.ptr(dout), _lib.ptr(gate), _lib.ptr(up), _lib.ptr(dgate), _lib.ptr(dup), c_ll(dout.stride(0)),
+                                          c_ll(gate.stride(0)), c_ll(up.stride(0)), c_ll(rows), c_ll(n), c_int(DTYPE_CODE[gate.dtype]),
+                                          c_int(ACTIVATION_CODE[activation]), c_int(_lib.sm_count(gate.device)), _lib.stream_ptr())
+    _lib.check_rc(rc, "sb_gated_product_bwd")
+    _lib.count(1)
+    return dgate, dup
+
+
+def rotary(q, k, inv_freq: torch.Tensor, positions, first: int, interleaved: bool, scale: float, sign: float):
+    """Rotated copies of ``q`` ``[B, S, H, D]`` and ``k`` (either may be ``None``), contiguous.
+
+    ``positions`` is an int32 / int64 ``[B, S]`` tensor of any strides, or ``None`` for ``first + s``.
+    """
+    some = q if q is not None else k
+    b, s, _, d = some.shape
+    oq = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    strides = (c_ll * 6)(*(q.stride()[:3] if q is not None else (0, 0, 0)), *(k.stride()[:3] if k is not None else (0, 0, 0)))
+    pb, ps = (0, 0) if positions is None else positions.stride()
+    rc = _lib.load().sb_rotary(_lib.ptr(q), _lib.ptr(k), _lib.ptr(oq), _lib.ptr(ok), strides, _lib.ptr(inv_freq), _lib.ptr(positions),
+                               c_int(int(positions is not None and positions.dtype == torch.int64)), c_ll(pb), c_ll(ps), c_ll(first), c_ll(b), c_int(s),
+                               c_int(0 if q is None else q.shape[2]), c_int(0 if k is None else k.shape[2]), c_int(d), c_int(2 * inv_freq.numel()),
+                               c_int(int(interleaved)), c_int(DTYPE_CODE[some.dtype]), c_float(scale), c_float(sign),
+                               c_int(_lib.sm_count(some.device)), _lib.stream_ptr())
+    _lib.check_rc(rc, "sb_rotary")
+    _lib.count(1)
+    return oq, ok

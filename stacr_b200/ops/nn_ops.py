@@ -8,7 +8,10 @@ the framework ops, which are also the oracles of the kernel tests.
 
 from __future__ import annotations
 
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from . import _lib
@@ -441,3 +444,324 @@ def rotary_qk_supported(qkv: torch.Tensor, head_dim: int, rot: int) -> bool:
 def rotary_qk(qkv, cos_half, sin_half, seq: int, heads: int, head_dim: int, rot: int):
     """``qkv``: ``[B, S, heads * 3 * head_dim]`` bf16 (per-head interleaved q|k|v); tables ``[S, rot/2]`` fp32."""
     return _RotaryQKFn.apply(qkv, cos_half, sin_half, seq, heads, head_dim, rot)
+
+
+# ------------------------------------------------------------------------------ rotary positions of separate q and k
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None, *, seq_len: int | None = None, device=None):
+    """``(inv_freq, scale)`` for :func:`rotary`: ``dim / 2`` angular frequencies in 64 bits and the factor on the rotated values.
+
+    ``scaling`` stretches the frequencies to contexts longer than the trained one; its ``rope_type`` (or ``type``) is
+
+    * ``default``: none;
+    * ``linear``: every frequency divided by ``factor`` (position interpolation);
+    * ``ntk``: the base raised to ``base * factor^(dim / (dim - 2))``, which divides the lowest frequency by ``factor`` and leaves the highest;
+    * ``dynamic``: the same with the factor that ``seq_len`` needs, ``factor * seq_len / original - (factor - 1)``, beyond the original length;
+    * ``yarn``: divided by ``factor`` where fewer than ``beta_slow`` turns fit into the original length, kept where more than ``beta_fast``
+      do, linear in between; ``scale = 0.1 ln(factor) + 1`` unless ``attention_factor`` is given;
+    * ``llama3``: divided where the wavelength exceeds ``original / low_freq_factor``, kept below ``original / high_freq_factor``, and
+      blended in between.
+
+    ``original`` is ``original_max_position_embeddings``.
+    """
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"rotary dimension must be positive and even, got {dim}")
+    if base <= 0:
+        raise ValueError(f"rotary base must be positive, got {base}")
+    index = torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim
+    inv = float(base) ** -index
+    scaling = scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind in (None, "default"):
+        return inv, 1.0
+    if kind not in ("linear", "ntk", "dynamic", "yarn", "llama3"):
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    if "factor" not in scaling:
+        raise ValueError(f"rotary scaling {kind!r} needs a factor")
+    factor = float(scaling["factor"])
+    if factor < 1:
+        raise ValueError(f"rotary scaling factor must be at least 1, got {factor}")
+    original = scaling.get("original_max_position_embeddings")
+    if kind in ("dynamic", "yarn", "llama3") and not original:
+        raise ValueError(f"rotary scaling {kind!r} needs original_max_position_embeddings")
+    if kind == "linear":
+        return inv / factor, 1.0
+    if kind in ("ntk", "dynamic"):
+        if kind == "dynamic":
+            factor = factor * seq_len / original - (factor - 1) if seq_len is not None and seq_len > original else 1.0
+        stretched = float(base) * factor ** (dim / (dim - 2)) if dim > 2 else float(base)
+        return stretched ** -index, 1.0
+    if kind == "yarn":
+        def pair_with(turns):       # the (real) pair index whose frequency makes this many turns over the original length
+            return dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low = max(math.floor(pair_with(float(scaling.get("beta_fast", 32)))), 0)
+        high = min(math.ceil(pair_with(float(scaling.get("beta_slow", 1)))), dim - 1)
+        ramp = ((torch.arange(dim // 2, dtype=torch.float64, device=device) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        attention = scaling.get("attention_factor")
+        return inv / factor * ramp + inv * (1 - ramp), float(attention) if attention is not None else 0.1 * math.log(factor) + 1.0
+    low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+    if high <= low:
+        raise ValueError(f"high_freq_factor must exceed low_freq_factor, got {high} and {low}")
+    blend = ((original * inv / (2 * math.pi) - low) / (high - low)).clamp(0, 1)      # wavelengths in the original length
+    return inv / factor * (1 - blend) + inv * blend, 1.0
+
+
+def _rotary_reference(x, angle, interleaved: bool, scale: float):
+    """The framework-op form of :func:`rotary` for one tensor: ``angle`` is ``[B or 1, S, rot / 2]`` in 64 bits."""
+    wide = x.dtype if x.dtype in (torch.float32, torch.float64) else torch.float32
+    cos, sin = (scale * angle.cos()).to(wide)[:, :, None], (scale * angle.sin()).to(wide)[:, :, None]
+    rot = 2 * angle.shape[-1]
+    r, rest = x[..., :rot].to(wide), x[..., rot:]
+    a, b = (r[..., 0::2], r[..., 1::2]) if interleaved else r.chunk(2, dim=-1)
+    y = (a * cos - b * sin, b * cos + a * sin)
+    y = torch.stack(y, dim=-1).flatten(-2) if interleaved else torch.cat(y, dim=-1)
+    return torch.cat((y.to(x.dtype), rest), dim=-1)
+
+
+class _RotaryFn(torch.autograd.Function):
+    """The rotation of q and k; its gradient is the rotation by the opposite angle of the outputs' gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, positions, first, interleaved, scale):
+        from . import nn_kernels
+
+        ctx.save_for_backward(inv_freq, positions)
+        ctx.set_materialize_grads(False)
+        ctx.first, ctx.interleaved, ctx.scale = first, interleaved, scale
+        with _lib.on_device(q):
+            return nn_kernels.rotary(_heads(q), _heads(k), inv_freq, positions, first, interleaved, scale, 1.0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        from . import nn_kernels
+
+        inv_freq, positions = ctx.saved_tensors
+        gq = _heads(gq) if ctx.needs_input_grad[0] else None
+        gk = _heads(gk) if ctx.needs_input_grad[1] else None
+        if gq is not None or gk is not None:
+            with _lib.on_device(inv_freq):
+                gq, gk = nn_kernels.rotary(gq, gk, inv_freq, positions, ctx.first, ctx.interleaved, ctx.scale, -1.0)
+        return gq, gk, None, None, None, None, None
+
+
+def _heads(t):
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: float = 1.0):
+    """Rotary positions: ``(q', k')`` for ``q`` ``[B, S, heads, D]`` and ``k`` ``[B, S, kv_heads, D]`` (or ``None``).
+
+    ``inv_freq`` (see :func:`rotary_frequencies`) has ``rot / 2`` angular frequencies; the first ``rot <= D`` values of a head are
+    turned, as pairs ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)``, and the rest is copied.  Pair ``i`` at position ``p`` is
+    turned by ``p * inv_freq[i]`` and multiplied by ``scale``; the angle is formed in 64 bits.  ``positions`` is ``None`` (``0 .. S-1``),
+    an int (the first token's position), or an integer tensor ``[S]``, ``[1, S]``, ``[B, 1]`` or ``[B, S]``.  Inputs may have any strides
+    (a transposed ``[B, heads, S, D]`` view is read in place); results are contiguous.
+    """
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("rotary expects q and k as [batch, sequence, heads, head_dim]")
+    b, s, _, d = q.shape
+    if k is not None and (k.shape[0] != b or k.shape[1] != s or k.shape[3] != d):
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, sequence or head_dim")
+    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+        raise ValueError("q and k must have one dtype and one device")
+    if not q.is_floating_point():
+        raise TypeError(f"rotary expects floating-point heads, got {q.dtype}")
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 0 < 2 * inv_freq.numel() <= d:
+        raise ValueError(f"inv_freq must hold 1 to {d // 2} frequencies, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    first = 0
+    if isinstance(positions, int):
+        first, positions = positions, None
+    elif positions is not None:
+        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+            raise TypeError(f"positions must be integers, got {positions.dtype}")
+        if positions.dim() not in (1, 2) or positions.shape[-1] not in (1, s) or (positions.dim() == 2 and positions.shape[0] not in (1, b)):
+            raise ValueError(f"positions {tuple(positions.shape)} do not fit [{b}, {s}]")
+        positions = positions.to(q.device).expand(b, s)
+    inv = inv_freq.detach().to(device=q.device, dtype=torch.float64).contiguous()
+    if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and q.numel() + (0 if k is None else k.numel()) > 0 and _lib.available():
+        if positions is not None and positions.dtype not in (torch.int32, torch.int64):
+            positions = positions.to(torch.int64)
+        return _RotaryFn.apply(q, k, inv, positions, first, bool(interleaved), float(scale))
+    where = torch.arange(first, first + s, device=q.device)[None] if positions is None else positions
+    angle = where.to(torch.float64)[..., None] * inv
+    return _rotary_reference(q, angle, interleaved, scale), None if k is None else _rotary_reference(k, angle, interleaved, scale)
+
+
+# ------------------------------------------------------------------------------ gated activation
+_ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda x: F.gelu(x, approximate="tanh")}
+
+
+def _check_activation(activation: str) -> None:
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}; choose from {sorted(_ACTIVATIONS)}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as a matrix with contiguous columns: a view where its strides allow one, else a copy."""
+    n = t.shape[-1]
+    if t.stride(-1) == 1 or n == 1:
+        try:
+            return t.view(-1, n) if t.dim() != 2 else t
+        except RuntimeError:
+            pass
+    return t.reshape(-1, n).contiguous()
+
+
+def _flat_rows(*ts: torch.Tensor):
+    """The matrices as one row when all are contiguous: widths that are no multiple of a vector then cost only the last few elements."""
+    if all(t.is_contiguous() for t in ts):
+        return tuple(t.view(1, -1) for t in ts)
+    return ts
+
+
+class _GatedProductFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up, activation):
+        from . import nn_kernels
+
+        ctx.save_for_backward(gate, up)
+        ctx.activation = activation
+        with _lib.on_device(gate):
+            g2, u2 = _flat_rows(_rows(gate), _rows(up))
+            return nn_kernels.gated_product_fwd(g2, u2, activation).view(gate.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        from . import nn_kernels
+
+        gate, up = ctx.saved_tensors
+        with _lib.on_device(gate):
+            d2, g2, u2 = _flat_rows(_rows(dout), _rows(gate), _rows(up))
+            dgate, dup = nn_kernels.gated_product_bwd(d2, g2, u2, ctx.activation, *ctx.needs_input_grad[:2])
+        return None if dgate is None else dgate.view(gate.shape), None if dup is None else dup.view(up.shape), None
+
+
+def gated_product(gate, up, activation: str = "silu"):
+    """``act(gate) * up`` for two tensors of one shape, in fp32 and rounded once; ``activation``: ``silu``, ``gelu`` or ``gelu_tanh``.
+
+    bf16, fp16 and fp32 CUDA tensors take one kernel forward and one backward; rows may be strided (the halves of one fused
+    projection).  Elsewhere, and for mixed types, the framework ops.
+    """
+    _check_activation(activation)
+    if gate.shape != up.shape:
+        raise ValueError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} differ in shape")
+    if (gate.is_cuda and gate.device == up.device and gate.dtype == up.dtype and gate.dtype in (torch.bfloat16, torch.float16, torch.float32)
+            and gate.numel() > 0 and gate.dim() > 0 and _lib.available()):
+        return _GatedProductFn.apply(gate, up, activation)
+    return _ACTIVATIONS[activation](gate) * up
+
+
+# ------------------------------------------------------------------------------ gated feed-forward: both projections and the product
+def _take_slot(weight):
+    """The fp32 buffer a gradient synchroniser has lent for this weight's gradient, or ``None``."""
+    slot = getattr(weight, "_sb_grad_out", None) if getattr(weight, "_sb_grad_fresh", False) else None
+    if slot is None or slot.dtype != torch.float32 or weight.dtype != torch.float32:
+        return None
+    weight._sb_grad_fresh = False
+    return slot
+
+
+def _hand_over(weight, dw, slot):
+    """What goes back through autograd for a weight whose gradient ``dw`` was written, into ``slot`` if there is one."""
+    ready = getattr(weight, "_sb_grad_ready", None) if slot is not None else None
+    if ready is not None and not getattr(weight, "_sb_tied", False):
+        ready()
+        return None
+    return dw if dw.dtype == weight.dtype else dw.to(weight.dtype)
+
+
+def _bf16_operand(weight):
+    from ..layers import _bf16_weight
+
+    return _bf16_weight(weight).contiguous()
+
+
+class _GatedLinearFn(torch.autograd.Function):
+    """``h = act(x Wg^T + bg) * (x Wu^T + bu)`` on bf16 operands.
+
+    Kept for backward: x, and the two projections in bf16 (what two separate linear layers would keep, without the activation)
+    unless ``recompute``, which forms them again from x: a third less memory traffic is not the point, the two ``[tokens, F]``
+    matrices not being held between the passes is.
+    """
+
+    @staticmethod
+    def forward(ctx, x2d, gate_weight, up_weight, gate_bias, up_bias, activation, recompute):
+        from . import gated
+
+        with _lib.on_device(x2d):
+            xa = (x2d if x2d.dtype == torch.bfloat16 else x2d.to(torch.bfloat16)).contiguous()
+            h, g, u = gated.forward(xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), activation,
+                                    keep=not recompute)
+        ctx.save_for_backward(xa, gate_weight, up_weight, gate_bias, up_bias, g, u)
+        ctx.activation, ctx.in_dtype = activation, x2d.dtype
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        from . import gated, stacr_ops
+
+        xa, gate_weight, up_weight, gate_bias, up_bias, g, u = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dwg = dwu = dbg = dbu = None
+        with _lib.on_device(xa):
+            d = (dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16)).contiguous()
+            wg, wu = _bf16_operand(gate_weight), _bf16_operand(up_weight)
+            if g is None:
+                dg, du = gated.backward_recomputed(d, xa, wg, wu, _f32_bias(gate_bias), _f32_bias(up_bias), ctx.activation)
+            else:
+                dg, du = gated.backward_kept(d, g, u, ctx.activation)
+            if need[0]:
+                dx = gated.input_gradient(dg, du, wg, wu).to(ctx.in_dtype)
+            if need[1] or need[2]:
+                same = gate_weight is up_weight       # one weight in both places receives two gradients: neither may use its slot
+                slots = [None if same or not need[i + 1] else _take_slot(w) for i, w in enumerate((gate_weight, up_weight))]
+                dwg, dwu = gated.weight_gradients(dg, du, xa, gate_weight.dtype, up_weight.dtype, slots, need[1], need[2])
+                dwg = None if dwg is None else _hand_over(gate_weight, dwg, slots[0])
+                dwu = None if dwu is None else _hand_over(up_weight, dwu, slots[1])
+            if gate_bias is not None and need[3]:
+                dbg = stacr_ops.colsum(dg).to(gate_bias.dtype)
+            if up_bias is not None and need[4]:
+                dbu = stacr_ops.colsum(du).to(up_bias.dtype)
+        return dx, dwg, dwu, dbg, dbu, None, None
+
+
+def _f32_bias(bias):
+    return None if bias is None else bias.detach().float().contiguous()
+
+
+def gated_linear_supported(x, gate_weight, up_weight) -> bool:
+    """Whether :func:`gated_linear` takes its kernels for these operands (bf16 activations, or bf16 autocast, on one GPU)."""
+    return (x.is_cuda and x.device == gate_weight.device == up_weight.device and gate_weight.dim() == 2 and x.shape[-1] % 8 == 0
+            and gate_weight.shape[0] % 8 == 0 and x.numel() > 0 and gate_weight.numel() > 0 and _lib.available()
+            and (x.dtype == torch.bfloat16 or (torch.is_autocast_enabled() and torch.get_autocast_dtype("cuda") == torch.bfloat16)))
+
+
+def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, activation: str = "silu", recompute: bool = False):
+    """``act(x Wg^T + bg) * (x Wu^T + bu)``: the first half of a gated feed-forward block, ``[..., K]`` to ``[..., F]``.
+
+    Weights are ``[F, K]``; ``activation``: ``silu``, ``gelu`` or ``gelu_tanh``.  bf16 activations (or bf16 autocast) on a GPU with
+    ``K`` and ``F`` multiples of 8 run on tensor cores, projections, activation and product in one kernel; elsewhere the framework ops.
+    Backward keeps the two projections, or with ``recompute`` only ``x`` and forms them again.
+    """
+    _check_activation(activation)
+    if gate_weight.dim() != 2 or gate_weight.shape != up_weight.shape or x.dim() < 1 or x.shape[-1] != gate_weight.shape[1]:
+        raise ValueError(f"weights {tuple(gate_weight.shape)} and {tuple(up_weight.shape)} do not project x {tuple(x.shape)}")
+    for bias in (gate_bias, up_bias):
+        if bias is not None and tuple(bias.shape) != (gate_weight.shape[0],):
+            raise ValueError(f"bias {tuple(bias.shape)} does not fit {gate_weight.shape[0]} outputs")
+    if not gated_linear_supported(x, gate_weight, up_weight):
+        return gated_product(linear(x, gate_weight, gate_bias), linear(x, up_weight, up_bias), activation)
+    x2d = x.reshape(-1, x.shape[-1])
+    leaves = (x, gate_weight, up_weight, gate_bias, up_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+        h = _GatedLinearFn.apply(x2d, gate_weight, up_weight, gate_bias, up_bias, activation, bool(recompute))
+    else:
+        from . import gated
+
+        with _lib.on_device(x):
+            h = gated.forward(x2d.detach().to(torch.bfloat16).contiguous(), _bf16_operand(gate_weight), _bf16_operand(up_weight),
+                              _f32_bias(gate_bias), _f32_bias(up_bias), activation, keep=False)[0]
+    return h.reshape(*x.shape[:-1], gate_weight.shape[0])

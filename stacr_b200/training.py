@@ -19,6 +19,7 @@ from typing import Any, NamedTuple
 
 import torch
 
+from .optim import clip_grad_norm_
 from .surgery import _SELECTION_KEYS, apply_stacr, select_target_names, set_step
 from .utils import device_from_config, set_seed, write_csv
 
@@ -385,7 +386,7 @@ def train_model(model, train_batches, config: dict, *, validation_batches=None) 
                 tokens += int(batch.get("attention_mask", torch.ones_like(batch["input_ids"])).sum())
         if cfg.get("max_grad_norm") is not None:
             scaler.unscale_(optimizer)
-            torch.nn.utils.clip_grad_norm_(model.parameters(), float(cfg["max_grad_norm"]))
+            clip_grad_norm_(model.parameters(), float(cfg["max_grad_norm"]))
         scaler.step(optimizer)
         scaler.update()
         if device.type == "cuda":
