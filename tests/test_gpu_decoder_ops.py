@@ -204,8 +204,8 @@ def gated_exact(x, wg, wu, bg, bu, dh, act):
 def gated_bounds(x, wg, wu, bg, bu, dh, act, g, u, keep):
     """Bounds of (h, dx, dWg, dWu, dbg, dbu), element by element.
 
-    A projection is off by its fp32 summation, at most (K + 2) 2^-24 times the sum of its terms' sizes, and by half a bf16 step more
-    where it is kept for backward.  |act'| <= 1.13, |act''| <= 1.  The derivative's products are rounded to bf16 before they are
+    A projection is off by its fp32 summation, at most (K + 2) 2^-24 times the sum of its terms' sizes; |act'| <= 1.13, |act''| <= 1.
+    The factors that are kept for backward have 24 bits (half a step: 2^-16).  The derivative's products are rounded to bf16 before they are
     multiplied again; sums over F or the tokens in fp32 add their length times 2^-24; every result is rounded once.
     """
     e, f32 = HALF[torch.bfloat16], 2.0 ** -24
@@ -220,11 +220,10 @@ def gated_bounds(x, wg, wu, bg, bu, dh, act, g, u, keep):
     a, da, U = a.detach().abs(), da.abs(), u.abs()
     fp = 16 * f32 * g.abs().clamp_min(1.2)
     bh = (a * U) * e + (1.13 * eg + fp) * (U + eu) + a * eu + 1e-30
-    if keep:
-        eg, eu = eg + e * (g.abs() + eg), eu + e * (U + eu)
     ea, eda = 1.13 * eg + fp, eg + fp
-    edg = D * ((eda * (U + eu)) + da * eu)
-    edu = D * ea
+    kept = 2.0 ** -16 if keep else 0.0
+    edg = D * ((eda * (U + eu)) + da * eu + kept * (U + eu) * (da + eda))
+    edu = D * (ea + kept * (a + ea))
     DG, DU = D * U * da, D * a
     edg, edu = edg + e * (DG + edg) + 1e-35, edu + e * (DU + edu) + 1e-35
     f = WG.shape[0]
