@@ -189,9 +189,37 @@ def sm_count(device=None) -> int:
     return max(1, _sms[idx] - _reserved_sms)
 
 
+_ENTRIES: dict = {}
+_LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
+
+
+def entry(name: str, letters: str):
+    """An entry point with declared argument types (one letter each: pointer, int, long long, float, double).
+
+    Plain Python numbers then convert by themselves, which costs a launch several microseconds less than wrapping each in a
+    ctypes object; small calls are bound by the host.
+    """
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = getattr(load(), name)
+        fn.argtypes, fn.restype = [_LETTERS[c] for c in letters], ctypes.c_int
+        _ENTRIES[name] = fn
+    return fn
+
+
 def on_device(t: torch.Tensor):
-    """Context in which the current device, and with it the stream that :func:`stream_ptr` returns, is the tensor's."""
-    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    """Context in which the current device is the tensor's: a launch goes to the current device, whatever stream it names."""
+    return _HERE_ALREADY if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def place(t: torch.Tensor) -> tuple[int, int]:
+    """``(SM count, raw handle of the current stream)`` of the tensor's device."""
+    index = t.get_device()
+    sms = _sms.get(index)
+    return (sm_count(t.device) if sms is None else max(1, sms - _reserved_sms)), (_raw_stream(index) if _raw_stream is not None else stream_ptr())
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -476,46 +476,26 @@ __global__ void __launch_bounds__(256) gated_factors_kernel(const uint4* __restr
 }  // namespace gg
 }  // namespace sb
 
-// h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) in bf16; x [M, K], weights [F, K] contiguous; K and F multiples of 8.
-// a_hi, b_hi [M, F] 16-bit and a_lo, b_lo [M, ceil16(F)] 8-bit receive the backward's factors unless a_hi is null.
-extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, void* a_hi, void* a_lo, void* b_hi,
-                                void* b_lo, int M, int K, int F, int act, int sms, int* status, void* stream) {
-  using namespace sb;
-  if (M <= 0 || K <= 0 || F <= 0 || K % 8 || F % 8) return -2;
-  if (!gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(h) || !gg::aligned16(a_hi) || !gg::aligned16(a_lo) ||
-      !gg::aligned16(b_hi) || !gg::aligned16(b_lo))
-    return -3;
+namespace sb {
+namespace gg {
+
+// what every entry asks for: operands on 16 bytes, K and F multiples of 8 (rows of 16 bytes, as TMA and the vector stores need them)
+static bool proper(int M, int K, int F) { return M > 0 && K > 0 && F > 0 && K % 8 == 0 && F % 8 == 0; }
+
+template <int MODE>
+static int project(const void* x, const void* wg, const void* wu, Params& p, int act, int sms, cudaStream_t st) {
   CUtensorMap ta, tg, tu;
-  int rc = make_tensor_map_bf16(&ta, x, K, M, K, gg::HM);
-  if (!rc) rc = make_tensor_map_bf16(&tg, wg, K, F, K, gg::HM);
-  if (!rc) rc = make_tensor_map_bf16(&tu, wu, K, F, K, gg::HM);
-  if (rc) return rc;
-  gg::Params p{M, F, K, 1, {0, 0}, F, (F + 15) / 16 * 16, {h, nullptr}, {bg, bu}, nullptr, static_cast<unsigned short*>(a_hi), static_cast<unsigned short*>(b_hi),
-               static_cast<unsigned char*>(a_lo), static_cast<unsigned char*>(b_lo), status};
-  return gg::launch_act<gg::FORWARD>(act, ta, ta, tg, tu, p, sms, static_cast<cudaStream_t>(stream));
+  int rc = make_tensor_map_bf16(&ta, x, p.K, p.M, p.K, HM);
+  if (!rc) rc = make_tensor_map_bf16(&tg, wg, p.K, p.N, p.K, HM);
+  if (!rc) rc = make_tensor_map_bf16(&tu, wu, p.K, p.N, p.K, HM);
+  return rc ? rc : launch_act<MODE>(act, ta, ta, tg, tu, p, sms, st);
 }
 
-// dG, dU [M, F] from dh [M, F] with the projections formed again.
-extern "C" int sb_gated_recompute(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, const void* dh, void* dg, void* du, int M,
-                                  int K, int F, int act, int sms, int* status, void* stream) {
-  using namespace sb;
-  if (M <= 0 || K <= 0 || F <= 0 || K % 8 || F % 8) return -2;
-  if (!gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(dh) || !gg::aligned16(dg) || !gg::aligned16(du)) return -3;
-  CUtensorMap ta, tg, tu;
-  int rc = make_tensor_map_bf16(&ta, x, K, M, K, gg::HM);
-  if (!rc) rc = make_tensor_map_bf16(&tg, wg, K, F, K, gg::HM);
-  if (!rc) rc = make_tensor_map_bf16(&tu, wu, K, F, K, gg::HM);
-  if (rc) return rc;
-  gg::Params p{M, F, K, 1, {0, 0}, F, 0, {dg, du}, {bg, bu}, static_cast<const __nv_bfloat16*>(dh), nullptr, nullptr, nullptr, nullptr, status};
-  return gg::launch_act<gg::RECOMPUTE>(act, ta, ta, tg, tu, p, sms, static_cast<cudaStream_t>(stream));
-}
-
-// dG, dU [M, F] from dh and the factors kept by sb_gated_forward.
-extern "C" int sb_gated_factors(const void* dh, const void* a_hi, const void* a_lo, const void* b_hi, const void* b_lo, void* dg, void* du, int M, int F, int sms,
-                                void* stream) {
-  using namespace sb;
-  if (M <= 0 || F <= 0 || F % 8) return -2;
+// dG, dU [M, F] from dh and the kept factors
+static int factors(const void* dh, const unsigned short* hi, const unsigned char* lo, __nv_bfloat16* d, int M, int F, int sms, cudaStream_t st) {
   const int nv = F / 8;
+  const size_t mf = static_cast<size_t>(M) * F;
+  const long long ld_lo = (F + 15) / 16 * 16;
   int tx = 32;
   while (tx < 256 && tx < nv) tx <<= 1;
   const dim3 block(tx, 256 / tx);
@@ -523,46 +503,81 @@ extern "C" int sb_gated_factors(const void* dh, const void* a_hi, const void* a_
   const long long cap = (sms * 32ll + gx - 1) / gx, by = (M + static_cast<int>(block.y) - 1) / static_cast<int>(block.y);
   const long long lim = cap < 65535 ? cap : 65535;
   const dim3 grid(gx, static_cast<unsigned>(by < lim ? by : lim));
-  gg::gated_factors_kernel<<<grid, block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint4*>(dh), static_cast<const uint4*>(a_hi), static_cast<const unsigned char*>(a_lo), static_cast<const uint4*>(b_hi),
-      static_cast<const unsigned char*>(b_lo), static_cast<uint4*>(dg), static_cast<uint4*>(du), M, nv, (F + 15) / 16 * 16);
+  gated_factors_kernel<<<grid, block, 0, st>>>(static_cast<const uint4*>(dh), reinterpret_cast<const uint4*>(hi), lo, reinterpret_cast<const uint4*>(hi + mf),
+                                               lo + M * ld_lo, reinterpret_cast<uint4*>(d), reinterpret_cast<uint4*>(d + mf), M, nv, ld_lo);
   return static_cast<int>(cudaGetLastError());
 }
 
-// dx[M, K] = dG Wg + dU Wu in bf16; dG, dU [M, F], weights [F, K].
-extern "C" int sb_gated_input_grad(const void* dg, const void* du, const void* wg, const void* wu, void* dx, int M, int K, int F, int sms, int* status,
-                                   void* stream) {
-  using namespace sb;
-  if (M <= 0 || K <= 0 || F <= 0 || K % 8 || F % 8) return -2;
-  if (!gg::aligned16(dg) || !gg::aligned16(du) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(dx)) return -3;
+// dx[M, K] = dG Wg + dU Wu
+static int input_grad(const __nv_bfloat16* dg, const __nv_bfloat16* du, const void* wg, const void* wu, void* dx, int M, int K, int F, int sms, int* status,
+                      cudaStream_t st) {
   CUtensorMap a0, a1, b0, b1;
-  int rc = make_tensor_map_bf16(&a0, dg, F, M, F, gg::HM);
-  if (!rc) rc = make_tensor_map_bf16(&a1, du, F, M, F, gg::HM);
+  int rc = make_tensor_map_bf16(&a0, dg, F, M, F, HM);
+  if (!rc) rc = make_tensor_map_bf16(&a1, du, F, M, F, HM);
   if (!rc) rc = make_tensor_map_bf16(&b0, wg, K, F, K, 64);
   if (!rc) rc = make_tensor_map_bf16(&b1, wu, K, F, K, 64);
   if (rc) return rc;
-  gg::Params p{M, K, F, 1, {0, 0}, K, 0, {dx, nullptr}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
-  return gg::launch<gg::INPUT_GRAD, ACT_SILU>(a0, a1, b0, b1, p, sms, static_cast<cudaStream_t>(stream));
+  Params p{M, K, F, 1, {0, 0}, K, 0, {dx, nullptr}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
+  return launch<INPUT_GRAD, ACT_SILU>(a0, a1, b0, b1, p, sms, st);
 }
 
-// dWg = dG^T x and dWu = dU^T x [F, K], each fp32 or bf16; a null result is left out.
-extern "C" int sb_gated_weight_grads(const void* dg, const void* du, const void* x, void* dwg, void* dwu, int fp32_g, int fp32_u, int M, int K, int F, int sms,
-                                     int* status, void* stream) {
-  using namespace sb;
-  if (M <= 0 || K <= 0 || F <= 0 || K % 8 || F % 8) return -2;
-  if (!dwg && !dwu) return 0;
+// dWg = dG^T x and dWu = dU^T x [F, K], each fp32 or bf16; a null result is left out
+static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const void* x, void* dwg, void* dwu, int fp32_g, int fp32_u, int M, int K, int F,
+                        int sms, int* status, cudaStream_t st) {
   if (!dwg) {
     dg = du;
     dwg = dwu;
     fp32_g = fp32_u;
     dwu = nullptr;
   }
-  if (!gg::aligned16(dg) || !gg::aligned16(du) || !gg::aligned16(x) || !gg::aligned16(dwg) || !gg::aligned16(dwu)) return -3;
   CUtensorMap a0, a1, b;
   int rc = make_tensor_map_bf16(&a0, dg, F, M, F, 64);
   if (!rc) rc = make_tensor_map_bf16(&a1, dwu ? du : dg, F, M, F, 64);
   if (!rc) rc = make_tensor_map_bf16(&b, x, K, M, K, 64);
   if (rc) return rc;
-  gg::Params p{F, K, M, dwu ? 2 : 1, {fp32_g, fp32_u}, K, 0, {dwg, dwu}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
-  return gg::launch<gg::WEIGHT_GRAD, ACT_SILU>(a0, a1, b, b, p, sms, static_cast<cudaStream_t>(stream));
+  Params p{F, K, M, dwu ? 2 : 1, {fp32_g, fp32_u}, K, 0, {dwg, dwu}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
+  return launch<WEIGHT_GRAD, ACT_SILU>(a0, a1, b, b, p, sms, st);
+}
+
+}  // namespace gg
+}  // namespace sb
+
+// h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) in bf16; x [M, K], weights [F, K] contiguous; K and F multiples of 8.
+// hi [2, M, F] 16-bit and lo [2, M, ceil16(F)] 8-bit receive the backward's factors; both null: not kept.
+extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, void* hi, void* lo, int M, int K, int F,
+                                int act, int sms, int* status, void* stream) {
+  using namespace sb;
+  if (!gg::proper(M, K, F)) return -2;
+  if (!gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(h) || !gg::aligned16(hi) || !gg::aligned16(lo)) return -3;
+  const long long ld_lo = (F + 15) / 16 * 16;
+  unsigned short* ah = static_cast<unsigned short*>(hi);
+  unsigned char* al = static_cast<unsigned char*>(lo);
+  gg::Params p{M, F, K, 1, {0, 0}, F, ld_lo, {h, nullptr}, {bg, bu}, nullptr, ah, ah ? ah + static_cast<size_t>(M) * F : nullptr, al, al ? al + M * ld_lo : nullptr,
+               status};
+  return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, static_cast<cudaStream_t>(stream));
+}
+
+// d [2, M, F] = dG and dU, from the kept factors or (hi null) from the projections formed again; dx [M, K] unless null; the weight
+// gradients [F, K], each fp32 or bf16, unless null.
+extern "C" int sb_gated_backward(const void* dh, const void* x, const void* wg, const void* wu, const float* bg, const float* bu, const void* hi, const void* lo,
+                                 void* d, void* dx, void* dwg, void* dwu, int fp32_g, int fp32_u, int M, int K, int F, int act, int sms, int* status,
+                                 void* stream) {
+  using namespace sb;
+  if (!gg::proper(M, K, F)) return -2;
+  if (!gg::aligned16(dh) || !gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(hi) || !gg::aligned16(lo) || !gg::aligned16(d) ||
+      !gg::aligned16(dx) || !gg::aligned16(dwg) || !gg::aligned16(dwu))
+    return -3;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  __nv_bfloat16* dg = static_cast<__nv_bfloat16*>(d);
+  __nv_bfloat16* du = dg + static_cast<size_t>(M) * F;
+  int rc;
+  if (hi) {
+    rc = gg::factors(dh, static_cast<const unsigned short*>(hi), static_cast<const unsigned char*>(lo), dg, M, F, sms, st);
+  } else {
+    gg::Params p{M, F, K, 1, {0, 0}, F, 0, {dg, du}, {bg, bu}, static_cast<const __nv_bfloat16*>(dh), nullptr, nullptr, nullptr, nullptr, status};
+    rc = gg::project<gg::RECOMPUTE>(x, wg, wu, p, act, sms, st);
+  }
+  if (!rc && dx) rc = gg::input_grad(dg, du, wg, wu, dx, M, K, F, sms, status, st);
+  if (!rc && (dwg || dwu)) rc = gg::weight_grads(dg, du, x, dwg, dwu, fp32_g, fp32_u, M, K, F, sms, status, st);
+  return rc;
 }

@@ -149,13 +149,13 @@ static int rotary_typed(const RotaryArgs& a, int sms, cudaStream_t st) {
 
 // q [B, S, hq, D] and k [B, S, hk, D] (null with hk = 0) with the strides given, into contiguous oq, ok; dtype 0 bf16, 1 fp16, 2 fp32.
 // rot is even, 2 <= rot <= D.  sign +1 forward, -1 backward.
-extern "C" int sb_rotary(const void* q, const void* k, void* oq, void* ok, const long long* strides, const double* inv_freq, const void* positions,
-                         int pos64, long long pb, long long ps, long long first, long long B, int S, int hq, int hk, int D, int rot, int interleaved,
-                         int dtype, float scale, float sign, int sms, void* stream) {
+extern "C" int sb_rotary(const void* q, const void* k, void* oq, void* ok, long long qb, long long qs, long long qh, long long kb, long long ks, long long kh,
+                         const double* inv_freq, const void* positions, int pos64, long long pb, long long ps, long long first, long long B, int S, int hq,
+                         int hk, int D, int rot, int interleaved, int dtype, float scale, float sign, int sms, void* stream) {
   using namespace sb;
   if (B <= 0 || S <= 0 || hq + hk <= 0) return 0;
   if (rot < 2 || rot % 2 || rot > D || hq < 0 || hk < 0) return -2;
-  RotaryArgs a{q, k, oq, ok, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], inv_freq, positions, pb, ps, first,
+  RotaryArgs a{q, k, oq, ok, qb, qs, qh, kb, ks, kh, inv_freq, positions, pb, ps, first,
                B * S, S, hq, hk, D, rot, pos64, 0, scale, sign};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {

@@ -3,97 +3,47 @@ results ``[M, F]``; biases fp32 or ``None``; ``K`` and ``F`` multiples of 8."""
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .nn_kernels import ACTIVATION_CODE
-
-_TYPED = None
-
-
-def _typed_lib():
-    """The kernel library with the argument types of these entry points declared: plain Python numbers then convert by themselves."""
-    global _TYPED
-    if _TYPED is None:
-        lib = _lib.load()
-        vp, ci = ctypes.c_void_p, ctypes.c_int
-        for name, args in {"sb_gated_forward": [vp] * 10 + [ci] * 5 + [vp] * 2, "sb_gated_recompute": [vp] * 8 + [ci] * 5 + [vp] * 2,
-                           "sb_gated_factors": [vp] * 7 + [ci] * 3 + [vp], "sb_gated_input_grad": [vp] * 5 + [ci] * 4 + [vp] * 2,
-                           "sb_gated_weight_grads": [vp] * 5 + [ci] * 6 + [vp] * 2}.items():
-            getattr(lib, name).argtypes, getattr(lib, name).restype = args, ci
-        _TYPED = lib
-    return _TYPED
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _common(t):
-    return _lib.sm_count(t.device), _lib.status_word(t.device).data_ptr(), _lib.stream_ptr()
-
-
-def _done(rc: int, name: str) -> None:
-    _lib.check_rc(rc, name)
-    _lib.count(1)
-
-
 def forward(x, wg, wu, bg, bu, activation: str, keep: bool):
-    """``(h, kept)``: with ``keep`` the backward's two factors as ``(a_hi, a_lo, b_hi, b_lo)``, 16 and 8 bits of each value."""
+    """``(h, kept)``: with ``keep`` the backward's two factors, ``(hi [2, M, F], lo [2, M, F padded to 16])``, 16 and 8 bits of each value."""
     m, k = x.shape
     f = wg.shape[0]
-    h = torch.empty(m, f, dtype=torch.bfloat16, device=x.device)
-    kept = None
+    device = x.device
+    h = torch.empty((m, f), dtype=torch.bfloat16, device=device)
+    hi = lo = None
     if keep:
-        hi, lo = torch.empty(2, m, f, dtype=torch.int16, device=x.device), torch.empty(2, m, -(-f // 16) * 16, dtype=torch.uint8, device=x.device)
-        kept = hi[0], lo[0], hi[1], lo[1]      # every part starts on 16 bytes: f is a multiple of 8
-    a_hi, a_lo, b_hi, b_lo = (t.data_ptr() for t in kept) if keep else (None,) * 4
-    rc = _typed_lib().sb_gated_forward(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), a_hi, a_lo, b_hi, b_lo, m, k, f,
-                                       ACTIVATION_CODE[activation], *_common(x))
-    _done(rc, "sb_gated_forward")
-    return h, kept
+        hi, lo = torch.empty((2, m, f), dtype=torch.int16, device=device), torch.empty((2, m, (f + 15) // 16 * 16), dtype=torch.uint8, device=device)
+    sms, stream = _lib.place(x)
+    rc = _lib.entry("sb_gated_forward", "ppppppppiiiiipp")(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), _ptr(hi), _ptr(lo), m, k, f,
+                                                         ACTIVATION_CODE[activation], sms, _lib.status_word(device).data_ptr(), stream)
+    _lib.check_rc(rc, "sb_gated_forward")
+    _lib.count(1)
+    return h, ((hi, lo) if keep else None)
 
 
-def backward_kept(dh, a_hi, a_lo, b_hi, b_lo):
-    """``(dgate, dup)`` from what :func:`forward` kept."""
-    m, f = dh.shape
-    dg, du = torch.empty_like(dh), torch.empty_like(dh)
-    rc = _typed_lib().sb_gated_factors(dh.data_ptr(), a_hi.data_ptr(), a_lo.data_ptr(), b_hi.data_ptr(), b_lo.data_ptr(), dg.data_ptr(), du.data_ptr(), m, f,
-                                       _lib.sm_count(dh.device), _lib.stream_ptr())
-    _done(rc, "sb_gated_factors")
-    return dg, du
-
-
-def backward_recomputed(dh, x, wg, wu, bg, bu, activation: str):
-    """``(dgate, dup)`` with the projections formed again."""
+def backward(dh, x, wg, wu, bg, bu, activation: str, kept, need_dx: bool, out_gate, out_up):
+    """``(d, dx)``: ``d [2, M, F]`` holds dgate and dup, from what :func:`forward` kept or from the projections formed again, and
+    ``dx = dgate Wg + dup Wu``.  ``dgate^T x`` and ``dup^T x`` go to ``out_gate`` and ``out_up``, fp32 or bf16 ``[F, K]`` or ``None``."""
     m, k = x.shape
-    dg, du = torch.empty_like(dh), torch.empty_like(dh)
-    rc = _typed_lib().sb_gated_recompute(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), dh.data_ptr(), dg.data_ptr(), du.data_ptr(), m, k,
-                                         wg.shape[0], ACTIVATION_CODE[activation], *_common(x))
-    _done(rc, "sb_gated_recompute")
-    return dg, du
-
-
-def input_gradient(dg, du, wg, wu):
-    """``dgate Wg + dup Wu`` in bf16, summed in fp32."""
-    m, f = dg.shape
-    k = wg.shape[1]
-    dx = torch.empty(m, k, dtype=torch.bfloat16, device=dg.device)
-    rc = _typed_lib().sb_gated_input_grad(dg.data_ptr(), du.data_ptr(), wg.data_ptr(), wu.data_ptr(), dx.data_ptr(), m, k, f, *_common(dg))
-    _done(rc, "sb_gated_input_grad")
-    return dx
-
-
-def weight_gradients(dg, du, x, gate_dtype, up_dtype, slots, need_gate: bool, need_up: bool):
-    """``(dgate^T x, dup^T x)``, fp32 into a slot or for an fp32 weight, bf16 otherwise; ``None`` for one that is not needed."""
-    m, k = x.shape
-    out = []
-    for dtype, slot, need in ((gate_dtype, slots[0], need_gate), (up_dtype, slots[1], need_up)):
-        kind = torch.bfloat16 if dtype == torch.bfloat16 else torch.float32
-        out.append(None if not need else slot if slot is not None else torch.empty(dg.shape[1], k, dtype=kind, device=x.device))
-    rc = _typed_lib().sb_gated_weight_grads(dg.data_ptr(), du.data_ptr(), x.data_ptr(), _ptr(out[0]), _ptr(out[1]),
-                                            *(int(t is not None and t.dtype == torch.float32) for t in out), m, k, dg.shape[1], *_common(x))
-    _done(rc, "sb_gated_weight_grads")
-    return out
+    f = dh.shape[1]
+    device = x.device
+    d = torch.empty((2, m, f), dtype=torch.bfloat16, device=device)
+    dx = torch.empty((m, k), dtype=torch.bfloat16, device=device) if need_dx else None
+    hi, lo = kept if kept is not None else (None, None)
+    sms, stream = _lib.place(x)
+    rc = _lib.entry("sb_gated_backward", "pppppppppppp" + "iiiiiii" + "pp")(
+        dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), _ptr(hi), _ptr(lo), d.data_ptr(), _ptr(dx), _ptr(out_gate), _ptr(out_up),
+        out_gate is not None and out_gate.dtype == torch.float32, out_up is not None and out_up.dtype == torch.float32, m, k, f, ACTIVATION_CODE[activation], sms,
+        _lib.status_word(device).data_ptr(), stream)
+    _lib.check_rc(rc, "sb_gated_backward")
+    _lib.count(1 + int(need_dx) + int(out_gate is not None or out_up is not None))
+    return d, dx

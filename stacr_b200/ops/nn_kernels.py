@@ -184,10 +184,10 @@ ACTIVATION_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 def gated_product_fwd(gate: torch.Tensor, up: torch.Tensor, activation: str) -> torch.Tensor:
     """``act(gate) * up`` of two ``[rows, n]`` matrices with contiguous columns; the result is contiguous."""
     rows, n = gate.shape
-    out = torch.empty(rows, n, dtype=gate.dtype, device=gate.device)
-    rc = _lib.load().sb_gated_product_fwd(_lib.ptr(gate), _lib.ptr(up), _lib.ptr(out), c_ll(gate.stride(0)), c_ll(up.stride(0)), c_ll(rows), c_ll(n),
-                                          c_int(DTYPE_CODE[gate.dtype]), c_int(ACTIVATION_CODE[activation]), c_int(_lib.sm_count(gate.device)),
-                                          _lib.stream_ptr())
+    out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    rc = _lib.entry("sb_gated_product_fwd", "pppllll" + "iiip")(
+        gate.data_ptr(), up.data_ptr(), out.data_ptr(), gate.stride(0), up.stride(0), rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation],
+        *_lib.place(gate))
     _lib.check_rc(rc, "sb_gated_product_fwd")
     _lib.count(1)
     return out
@@ -196,11 +196,11 @@ def gated_product_fwd(gate: torch.Tensor, up: torch.Tensor, activation: str) -> 
 def gated_product_bwd(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activation: str, need_gate: bool = True, need_up: bool = True):
     """``(dgate, dup)`` of :func:`gated_product_fwd`, contiguous; ``None`` for one that is not needed."""
     rows, n = gate.shape
-    dgate = torch.empty(rows, n, dtype=gate.dtype, device=gate.device) if need_gate else None
-    dup = torch.empty(rows, n, dtype=gate.dtype, device=gate.device) if need_up else None
-    rc = _lib.load().sb_gated_product_bwd(_lib.ptr(dout), _lib.ptr(gate), _lib.ptr(up), _lib.ptr(dgate), _lib.ptr(dup), c_ll(dout.stride(0)),
-                                          c_ll(gate.stride(0)), c_ll(up.stride(0)), c_ll(rows), c_ll(n), c_int(DTYPE_CODE[gate.dtype]),
-                                          c_int(ACTIVATION_CODE[activation]), c_int(_lib.sm_count(gate.device)), _lib.stream_ptr())
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device) if need_gate else None
+    dup = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device) if need_up else None
+    rc = _lib.entry("sb_gated_product_bwd", "ppppplllll" + "iiip")(
+        dout.data_ptr(), gate.data_ptr(), up.data_ptr(), None if dgate is None else dgate.data_ptr(), None if dup is None else dup.data_ptr(), dout.stride(0),
+        gate.stride(0), up.stride(0), rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation], *_lib.place(gate))
     _lib.check_rc(rc, "sb_gated_product_bwd")
     _lib.count(1)
     return dgate, dup
@@ -213,15 +213,19 @@ def rotary(q, k, inv_freq: torch.Tensor, positions, first: int, interleaved: boo
     """
     some = q if q is not None else k
     b, s, _, d = some.shape
-    oq = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    strides = (c_ll * 6)(*(q.stride()[:3] if q is not None else (0, 0, 0)), *(k.stride()[:3] if k is not None else (0, 0, 0)))
-    pb, ps = (0, 0) if positions is None else positions.stride()
-    rc = _lib.load().sb_rotary(_lib.ptr(q), _lib.ptr(k), _lib.ptr(oq), _lib.ptr(ok), strides, _lib.ptr(inv_freq), _lib.ptr(positions),
-                               c_int(int(positions is not None and positions.dtype == torch.int64)), c_ll(pb), c_ll(ps), c_ll(first), c_ll(b), c_int(s),
-                               c_int(0 if q is None else q.shape[2]), c_int(0 if k is None else k.shape[2]), c_int(d), c_int(2 * inv_freq.numel()),
-                               c_int(int(interleaved)), c_int(DTYPE_CODE[some.dtype]), c_float(scale), c_float(sign),
-                               c_int(_lib.sm_count(some.device)), _lib.stream_ptr())
+    oq = ok = qp = kp = oqp = okp = pp = None
+    hq = hk = qb = qs = qh = kb = ks = kh = pb = ps = 0
+    if q is not None:
+        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        hq, (qb, qs, qh, _), qp, oqp = q.shape[2], q.stride(), q.data_ptr(), oq.data_ptr()
+    if k is not None:
+        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        hk, (kb, ks, kh, _), kp, okp = k.shape[2], k.stride(), k.data_ptr(), ok.data_ptr()
+    if positions is not None:
+        (pb, ps), pp = positions.stride(), positions.data_ptr()
+    rc = _lib.entry("sb_rotary", "pppp" + "llllll" + "ppi" + "llll" + "iiiiiii" + "ff" + "ip")(
+        qp, kp, oqp, okp, qb, qs, qh, kb, ks, kh, inv_freq.data_ptr(), pp, positions is not None and positions.dtype == torch.int64, pb, ps, first, b, s, hq, hk,
+        d, 2 * inv_freq.numel(), interleaved, DTYPE_CODE[some.dtype], scale, sign, *_lib.place(some))
     _lib.check_rc(rc, "sb_rotary")
     _lib.count(1)
     return oq, ok

@@ -577,12 +577,19 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
             raise TypeError(f"positions must be integers, got {positions.dtype}")
         if positions.dim() not in (1, 2) or positions.shape[-1] not in (1, s) or (positions.dim() == 2 and positions.shape[0] not in (1, b)):
             raise ValueError(f"positions {tuple(positions.shape)} do not fit [{b}, {s}]")
-        positions = positions.to(q.device).expand(b, s)
-    inv = inv_freq.detach().to(device=q.device, dtype=torch.float64).contiguous()
+        positions = (positions if positions.device == q.device else positions.to(q.device)).expand(b, s)
+    inv = inv_freq
+    if inv.dtype != torch.float64 or inv.device != q.device or inv.requires_grad or not inv.is_contiguous():
+        inv = inv.detach().to(device=q.device, dtype=torch.float64).contiguous()
     if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and q.numel() + (0 if k is None else k.numel()) > 0 and _lib.available():
         if positions is not None and positions.dtype not in (torch.int32, torch.int64):
             positions = positions.to(torch.int64)
-        return _RotaryFn.apply(q, k, inv, positions, first, bool(interleaved), float(scale))
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            return _RotaryFn.apply(q, k, inv, positions, first, bool(interleaved), float(scale))
+        from . import nn_kernels
+
+        with _lib.on_device(q):
+            return nn_kernels.rotary(_heads(q), _heads(k), inv, positions, first, bool(interleaved), float(scale), 1.0)
     where = torch.arange(first, first + s, device=q.device)[None] if positions is None else positions
     angle = where.to(torch.float64)[..., None] * inv
     return _rotary_reference(q, angle, interleaved, scale), None if k is None else _rotary_reference(k, angle, interleaved, scale)
@@ -615,16 +622,20 @@ def _flat_rows(*ts: torch.Tensor):
     return ts
 
 
+def _gated_product(gate, up, activation):
+    from . import nn_kernels
+
+    with _lib.on_device(gate):
+        g2, u2 = _flat_rows(_rows(gate), _rows(up))
+        return nn_kernels.gated_product_fwd(g2, u2, activation).view(gate.shape)
+
+
 class _GatedProductFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, activation):
-        from . import nn_kernels
-
         ctx.save_for_backward(gate, up)
         ctx.activation = activation
-        with _lib.on_device(gate):
-            g2, u2 = _flat_rows(_rows(gate), _rows(up))
-            return nn_kernels.gated_product_fwd(g2, u2, activation).view(gate.shape)
+        return _gated_product(gate, up, activation)
 
     @staticmethod
     @once_differentiable
@@ -649,7 +660,9 @@ def gated_product(gate, up, activation: str = "silu"):
         raise ValueError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} differ in shape")
     if (gate.is_cuda and gate.device == up.device and gate.dtype == up.dtype and gate.dtype in (torch.bfloat16, torch.float16, torch.float32)
             and gate.numel() > 0 and gate.dim() > 0 and _lib.available()):
-        return _GatedProductFn.apply(gate, up, activation)
+        if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+            return _GatedProductFn.apply(gate, up, activation)
+        return _gated_product(gate, up, activation)
     return _ACTIVATIONS[activation](gate) * up
 
 
@@ -673,6 +686,8 @@ def _hand_over(weight, dw, slot):
 
 
 def _bf16_operand(weight):
+    if weight.dtype == torch.bfloat16 and weight.is_contiguous():
+        return weight
     from ..layers import _bf16_weight
 
     return _bf16_weight(weight).contiguous()
@@ -704,26 +719,23 @@ class _GatedLinearFn(torch.autograd.Function):
 
         xa, gate_weight, up_weight, gate_bias, up_bias, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx = dwg = dwu = dbg = dbu = None
+        dbg = dbu = None
         with _lib.on_device(xa):
-            d = (dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16)).contiguous()
-            wg, wu = _bf16_operand(gate_weight), _bf16_operand(up_weight)
-            if kept:
-                dg, du = gated.backward_kept(d, *kept)
-            else:
-                dg, du = gated.backward_recomputed(d, xa, wg, wu, _f32_bias(gate_bias), _f32_bias(up_bias), ctx.activation)
-            if need[0]:
-                dx = gated.input_gradient(dg, du, wg, wu).to(ctx.in_dtype)
-            if need[1] or need[2]:
-                same = gate_weight is up_weight       # one weight in both places receives two gradients: neither may use its slot
-                slots = [None if same or not need[i + 1] else _take_slot(w) for i, w in enumerate((gate_weight, up_weight))]
-                dwg, dwu = gated.weight_gradients(dg, du, xa, gate_weight.dtype, up_weight.dtype, slots, need[1], need[2])
-                dwg = None if dwg is None else _hand_over(gate_weight, dwg, slots[0])
-                dwu = None if dwu is None else _hand_over(up_weight, dwu, slots[1])
+            dh = (dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16)).contiguous()
+            same = gate_weight is up_weight       # one weight in both places receives two gradients: neither may use its slot
+            slots = [None if same or not need[i + 1] else _take_slot(w) for i, w in enumerate((gate_weight, up_weight))]
+            dw = [None if not need[i + 1] else slots[i] if slots[i] is not None else
+                  torch.empty(w.shape, dtype=torch.bfloat16 if w.dtype == torch.bfloat16 else torch.float32, device=w.device)
+                  for i, w in enumerate((gate_weight, up_weight))]
+            d, dx = gated.backward(dh, xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), ctx.activation,
+                                   kept or None, need[0], *dw)
+            if dx is not None and dx.dtype != ctx.in_dtype:
+                dx = dx.to(ctx.in_dtype)
+            dwg, dwu = (None if g is None else _hand_over(w, g, slot) for w, g, slot in zip((gate_weight, up_weight), dw, slots))
             if gate_bias is not None and need[3]:
-                dbg = stacr_ops.colsum(dg).to(gate_bias.dtype)
+                dbg = stacr_ops.colsum(d[0]).to(gate_bias.dtype)
             if up_bias is not None and need[4]:
-                dbu = stacr_ops.colsum(du).to(up_bias.dtype)
+                dbu = stacr_ops.colsum(d[1]).to(up_bias.dtype)
         return dx, dwg, dwu, dbg, dbu, None, None
 
 
@@ -753,14 +765,14 @@ def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, act
             raise ValueError(f"bias {tuple(bias.shape)} does not fit {gate_weight.shape[0]} outputs")
     if not gated_linear_supported(x, gate_weight, up_weight):
         return gated_product(linear(x, gate_weight, gate_bias), linear(x, up_weight, up_bias), activation)
-    x2d = x.reshape(-1, x.shape[-1])
-    leaves = (x, gate_weight, up_weight, gate_bias, up_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
+    x2d = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad
+                                    or any(b is not None and b.requires_grad for b in (gate_bias, up_bias))):
         h = _GatedLinearFn.apply(x2d, gate_weight, up_weight, gate_bias, up_bias, activation, bool(recompute))
     else:
         from . import gated
 
         with _lib.on_device(x):
-            h = gated.forward(x2d.detach().to(torch.bfloat16).contiguous(), _bf16_operand(gate_weight), _bf16_operand(up_weight),
+            h = gated.forward((x2d if x2d.dtype == torch.bfloat16 else x2d.detach().to(torch.bfloat16)).contiguous(), _bf16_operand(gate_weight), _bf16_operand(up_weight),
                               _f32_bias(gate_bias), _f32_bias(up_bias), activation, keep=False)[0]
-    return h.reshape(*x.shape[:-1], gate_weight.shape[0])
+    return h if x.dim() == 2 else h.reshape(*x.shape[:-1], gate_weight.shape[0])

@@ -2,10 +2,9 @@
 
 from __future__ import annotations
 
-import ctypes
+from array import array
 from typing import Iterable
 
-import numpy as np
 import torch
 
 _KERNEL_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -29,48 +28,45 @@ def _dense(t: torch.Tensor) -> bool:
 
 def _kernel_table(grads):
     """``(pointers, sizes, type codes)`` of the distinct gradients, or ``None`` where the kernel does not apply."""
-    device = grads[0].device if grads else None
-    if device is None or device.type != "cuda":
+    if not grads or not grads[0].is_cuda:
         return None
-    for g in grads:
-        if type(g) is not torch.Tensor or g.device != device or g.dtype not in _KERNEL_DTYPES or g.layout != torch.strided or not _dense(g):
-            return None
+    device = grads[0].get_device()
     seen = {}
     for g in grads:
-        if g.numel():
-            seen.setdefault((g.data_ptr(), g.numel(), g.dtype), g)
-    ptrs = np.array([key[0] for key in seen], dtype=np.uint64)
-    sizes = np.array([key[1] for key in seen], dtype=np.int64)
-    codes = np.array([_KERNEL_DTYPES[key[2]] for key in seen], dtype=np.uint8)
-    order = np.argsort(ptrs, kind="stable")
-    ends = ptrs + sizes.astype(np.uint64) * np.where(codes == 2, 4, 2).astype(np.uint64)
-    if (ends[order][:-1] > ptrs[order][1:]).any():
-        raise ValueError("two gradients overlap in memory: clipping would scale the shared elements twice")
-    return ptrs, sizes, codes
+        code = _KERNEL_DTYPES.get(g.dtype)
+        if code is None or type(g) is not torch.Tensor or g.layout is not torch.strided or g.get_device() != device or not (g.is_contiguous() or _dense(g)):
+            return None
+        n = g.numel()
+        if n:
+            seen[g.data_ptr(), n, code] = None
+    end = 0
+    for start, n, code in sorted(seen):
+        if start < end:
+            raise ValueError("two gradients overlap in memory: clipping would scale the shared elements twice")
+        end = start + n * (4 if code == 2 else 2)
+    return [*zip(*seen)] if seen else ((), (), ())
 
 
 def _run(grads, table, max_norm: float | None) -> torch.Tensor:
     from ..ops import _lib
 
     ptrs, sizes, codes = table
-    device = grads[0].device
-    if not len(ptrs):
+    n, device = len(ptrs), grads[0].device
+    if not n:
         return torch.zeros((), dtype=torch.float32, device=device)
-    lib = _lib.load()
     with _lib.on_device(grads[0]):
-        sms = _lib.sm_count(device)
+        sms, stream = _lib.place(grads[0])
         norm = torch.empty((), dtype=torch.float32, device=device)
-        partial = torch.empty(lib.sb_clip_partials(ctypes.c_int(len(ptrs)), ctypes.c_int(sms)), dtype=torch.float64, device=device)
-        rc = lib.sb_grad_clip(ctypes.c_void_p(ptrs.ctypes.data), ctypes.c_void_p(sizes.ctypes.data), ctypes.c_void_p(codes.ctypes.data),
-                              ctypes.c_int(len(ptrs)), _lib.ptr(partial), _lib.ptr(norm), ctypes.c_double(0.0 if max_norm is None else max_norm),
-                              ctypes.c_int(int(max_norm is not None)), ctypes.c_int(sms), _lib.stream_ptr())
+        partial = torch.empty(_lib.entry("sb_clip_partials", "ii")(n, sms), dtype=torch.float64, device=device)
+        ptrs, sizes, codes = array("Q", ptrs), array("q", sizes), array("B", codes)
+        rc = _lib.entry("sb_grad_clip", "pppippdiip")(ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], n, partial.data_ptr(), norm.data_ptr(),
+                                                     0.0 if max_norm is None else max_norm, max_norm is not None, sms, stream)
     _lib.check_rc(rc, "sb_grad_clip")
-    groups = -(-len(ptrs) // lib.sb_clip_tensors_per_launch())
+    groups = -(-n // _lib.entry("sb_clip_tensors_per_launch", "")())
     _lib.count(groups + (1 if max_norm is None else groups))
     return norm
 
 
-@torch.no_grad()
 def grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor:
     """2-norm of all gradients together as a device scalar, without waiting for the device.  A gradient that occurs twice counts once."""
     grads = [p.grad for p in _parameters(parameters) if p.grad is not None]
@@ -80,7 +76,6 @@ def grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor
     return _run(grads, table, None)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and return their norm from before, as a device scalar.
@@ -103,6 +98,5 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped. "
                                "To disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
     norm = _run(grads, table, max_norm)
-    for g in grads:
-        torch.autograd.graph.increment_version(g)
+    torch.autograd.graph.increment_version(grads)
     return norm
