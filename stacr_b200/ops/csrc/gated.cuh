@@ -65,6 +65,12 @@ __device__ __forceinline__ void act_and_derivative(float x, float& act, float& d
   }
 }
 
+// Upper 24 bits of a float, rounded; NaN and infinity keep theirs.
+__device__ __forceinline__ unsigned upper24(float v) {
+  const unsigned b = __float_as_uint(v);
+  return (b & 0x7fffffffu) < 0x7f800000u ? b + 0x80u : b;
+}
+
 template <int ACT>
 __device__ __forceinline__ float activation(float x) {
   float act, der;

@@ -24,6 +24,11 @@ namespace sb {
 
 int make_tensor_map_bf16(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer);
 
+namespace gt {
+int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,
+            int act, cudaStream_t st);
+}
+
 namespace gg {
 
 using namespace g2;
@@ -52,12 +57,6 @@ struct Params {
   unsigned char *a_lo, *b_lo;
   int* status;
 };
-
-// Upper 24 bits of a float, rounded; NaN and infinity keep theirs.
-__device__ __forceinline__ unsigned upper24(float v) {
-  const unsigned b = __float_as_uint(v);
-  return (b & 0x7fffffffu) < 0x7f800000u ? b + 0x80u : b;
-}
 
 __device__ __forceinline__ void decode(int tile, int num_m, int num_n, int& m_blk, int& n_blk) {
   constexpr int G = 4;       // rows of tiles that run side by side: their x and weight tiles are shared through L2
@@ -545,13 +544,14 @@ static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const 
 // h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) in bf16; x [M, K], weights [F, K] contiguous; K and F multiples of 8.
 // hi [2, M, F] 16-bit and lo [2, M, ceil16(F)] 8-bit receive the backward's factors; both null: not kept.
 extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, void* hi, void* lo, int M, int K, int F,
-                                int act, int sms, int* status, void* stream) {
+                                int act, int tokens_max, int sms, int* status, void* stream) {
   using namespace sb;
-  if (!gg::proper(M, K, F)) return -2;
+  if (!gg::proper(M, K, F) || tokens_max > 64) return -2;
   if (!gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(h) || !gg::aligned16(hi) || !gg::aligned16(lo)) return -3;
   const long long ld_lo = (F + 15) / 16 * 16;
   unsigned short* ah = static_cast<unsigned short*>(hi);
   unsigned char* al = static_cast<unsigned char*>(lo);
+  if (M <= tokens_max) return gt::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, static_cast<cudaStream_t>(stream));
   gg::Params p{M, F, K, 1, {0, 0}, F, ld_lo, {h, nullptr}, {bg, bu}, nullptr, ah, ah ? ah + static_cast<size_t>(M) * F : nullptr, al, al ? al + M * ld_lo : nullptr,
                status};
   return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, static_cast<cudaStream_t>(stream));
