@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) gated_product_kernel(const GatedArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float act, der;
-          act_and_derivative<ACT>(to_f32(gv.v[i]), act, der);
+          act_and_derivative<ACT, false>(to_f32(gv.v[i]), act, der);
           const float dd = to_f32(dv.v[i]);
           o1.v[i] = from_f32<T>(dd * to_f32(uv.v[i]) * der);
           o2.v[i] = from_f32<T>(dd * act);

@@ -31,37 +31,30 @@ __device__ __forceinline__ float exp_f32(float x) {
   return fabsf(t) < 126.f ? fmaf(e * ln2, r, e) : e;
 }
 
-// 1 / (1 + e^-x).  e^-x overflows to infinity below x = -88, where the result is 0.
-__device__ __forceinline__ float sigmoid_f32(float x) { return __frcp_rn(1.f + exp_f32(-x)); }
-
-// tanh z = 1 - 2 / (1 + e^2z); |z| below 2^-3 would cancel, so the odd series z - z^3/3 + 2 z^5/15 - 17 z^7/315 (next term
-// 62 z^9/2835 < 2^-29 z) is used there.
-__device__ __forceinline__ float tanh_f32(float z) {
-  const float z2 = z * z;
-  const float series = z * fmaf(z2, fmaf(z2, fmaf(z2, -0.053968254f, 0.133333333f), -0.333333333f), 1.f);
-  return fabsf(z) < 0.125f ? series : 1.f - 2.f * __frcp_rn(1.f + exp_f32(2.f * z));
+// 1 / (1 + e^-x).  e^-x overflows to infinity below x = -88, where the result is 0.  FAST: the hardware's exponential and reciprocal,
+// off by (3 + 1.2 |x|) 2^-23 of the result: for results that are rounded to bf16 (2^-8) or kept in 24 bits (2^-16).
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_f32(float x) {
+  return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : __frcp_rn(1.f + exp_f32(-x));
 }
 
 // act(x) and act'(x):
-//   silu       x s,                        s (1 + x (1 - s)),      s = sigmoid(x)
-//   gelu       x Phi(x),                   Phi(x) + x phi(x)       (normal distribution function and density)
-//   gelu_tanh  x (1 + t) / 2,              (1 + t) / 2 + x (1 - t^2) w' / 2,   t = tanh w, w = sqrt(2/pi) (x + 0.044715 x^3)
-template <int ACT>
+//   silu       x s,        s (1 + x (1 - s)),               s = sigmoid(x)
+//   gelu       x Phi(x),   Phi(x) + x phi(x)                (normal distribution function and density)
+//   gelu_tanh  x s,        s (1 + x (1 - s) 2 w'),          s = sigmoid(2 w) = (1 + tanh w) / 2,  w = sqrt(2/pi) (x + 0.044715 x^3)
+template <int ACT, bool FAST>
 __device__ __forceinline__ void act_and_derivative(float x, float& act, float& der) {
-  if (ACT == ACT_SILU) {
-    const float s = sigmoid_f32(x);
-    act = x * s;
-    der = s * fmaf(x, 1.f - s, 1.f);
-  } else if (ACT == ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.707106781f * x);
-    const float pdf = 0.398942280f * exp_f32(-0.5f * x * x);
+  if (ACT == ACT_GELU) {
+    const float cdf = FAST ? 0.5f + 0.5f * erff(0.707106781f * x) : 0.5f * erfcf(-0.707106781f * x);
+    const float pdf = 0.398942280f * (FAST ? __expf(-0.5f * x * x) : exp_f32(-0.5f * x * x));
     act = x * cdf;
     der = fmaf(x, pdf, cdf);
   } else {
-    const float k = 0.797884561f, c = 0.044715f;
-    const float t = tanh_f32(k * x * fmaf(c * x, x, 1.f));
-    act = 0.5f * x * (1.f + t);
-    der = 0.5f * (1.f + t) + 0.5f * x * (1.f - t) * (1.f + t) * k * fmaf(3.f * c * x, x, 1.f);
+    const float k = 1.59576912f, c = 0.044715f;   // 2 sqrt(2/pi)
+    const float s = sigmoid_f32<FAST>(ACT == ACT_SILU ? x : k * x * fmaf(c * x, x, 1.f));
+    const float slope = ACT == ACT_SILU ? 1.f : k * fmaf(3.f * c * x, x, 1.f);
+    act = x * s;
+    der = s * fmaf(x * (1.f - s), slope, 1.f);
   }
 }
 
@@ -74,7 +67,7 @@ __device__ __forceinline__ unsigned upper24(float v) {
 template <int ACT>
 __device__ __forceinline__ float activation(float x) {
   float act, der;
-  act_and_derivative<ACT>(x, act, der);
+  act_and_derivative<ACT, false>(x, act, der);
   return act;
 }
 

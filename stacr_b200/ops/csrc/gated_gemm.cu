@@ -16,7 +16,7 @@
 // and the three bytes are the two factors' share of what separate layers keep (gate, act(gate), up in bf16: six bytes a feature).
 //
 // Pipeline, barriers and bounded waits are those of gemm_tc2.cu: a producer warp per CTA (TMA), one MMA thread in the even CTA,
-// four epilogue warps per CTA, six 32 KB stages, two accumulators so that a tile's epilogue runs under the next tile's main loop.
+// eight epilogue warps per CTA, five 32 KB stages, two accumulators so that a tile's epilogue runs under the next tile's main loop.
 #include "cta_pair.cuh"
 #include "gated.cuh"
 
@@ -35,11 +35,12 @@ using namespace g2;
 
 constexpr int TM = 256, TN = 256, TF = 128;  // accumulator of a CTA pair; features of a forward tile
 constexpr int HM = 128, BK = 64, UMMA_K = 16;
-constexpr int THREADS = 192;
+constexpr int EPI_WARPS = 8;                 // two per quarter of the tensor memory lanes, each with one half of the columns
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int A_BYTES = HM * BK * 2, STAGE_BYTES = 2 * A_BYTES;
-constexpr int STAGES = 6;
+constexpr int STAGES = 5;
 constexpr int WARP_EPI = 8192;               // staging of one epilogue warp
-constexpr int EPI_BYTES = 4 * WARP_EPI;
+constexpr int EPI_BYTES = EPI_WARPS * WARP_EPI;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 256;
 constexpr int TMEM_COLS = 512;
 
@@ -141,7 +142,7 @@ __device__ __forceinline__ void gated_chunk(const Params& p, const uint32_t (&vg
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float der;
-    act_and_derivative<ACT>(g[i], b[i], der);
+    act_and_derivative<ACT, true>(g[i], b[i], der);
     a[i] = u[i] * der;
   }
   float o[16];
@@ -201,7 +202,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 8);
+      mbar_init(&tmem_empty[a], 2 * EPI_WARPS);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -300,9 +301,9 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue warps (2..5) of both CTAs
-    const int quad = warp & 3;
-    uint8_t* st = epi_stage + quad * WARP_EPI;
+    // ------------------------------------------------------------ epilogue warps of both CTAs
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* st = epi_stage + (warp - 2) * WARP_EPI;
     int local = 0;
     bool ok = true;
     for (int tile = pair; tile < total_tiles && ok; tile += npairs, ++local) {
@@ -313,70 +314,81 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
       const uint32_t acc_ph = (local >> 1) & 1;
       const int row_base = m_blk * TM + static_cast<int>(crank) * HM + quad * 32;
       const int row = row_base + lane;
+      constexpr int CHUNKS = (PROJECT ? TF : TN) / 32;            // chunks of 16 columns in this warp's half
+      const int col_first = n_blk * STEP_N + half * CHUNKS * 16;
       if (!mbar_wait(&tmem_full[acc], acc_ph, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * TN;
-      if (PROJECT) {
-        // 32 features at a time: two 16-column chunks of both projections, staged and stored as row segments of 64 (32) bytes
-#pragma unroll 1
-        for (int c = 0; c < TF / 16; ++c) {
-          const int col0 = n_blk * TF + c * 16;
-          uint32_t vg[16], vu[16];
-          uint4 dh[2] = {};
-          tmem_ld_x16(t_row + c * 16, vg);
-          tmem_ld_x16(t_row + TF + c * 16, vu);
-          if (MODE == RECOMPUTE && row < p.M) {
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * TN + half * CHUNKS * 16;
+      if (row_base < p.M && col_first < p.N) {                     // the same for the whole warp
+        if (PROJECT) {
+          // 32 features at a time: two 16-column chunks of both projections, staged and stored as row segments of 64 (32) bytes.
+          // The next chunk is on its way from tensor memory while one is worked on.
+          uint32_t vg[2][16], vu[2][16];
+          tmem_ld_x16(t_row, vg[0]);
+          tmem_ld_x16(t_row + TF, vu[0]);
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-              if (col0 + q * 8 < p.N) dh[q] = __ldg(reinterpret_cast<const uint4*>(p.dh + static_cast<size_t>(row) * p.ld_hi + col0 + q * 8));
-          }
-          tmem_ld_wait();
-          gated_chunk<MODE, ACT>(p, vg, vu, dh, col0, lane, st, (c & 1) * 2);
-          if (c & 1) {
-            __syncwarp();
-            const int g0 = col0 - 16;
-            flush2(st, lane, p.out[0], p.ld_hi, row_base, p.M, g0, p.N);
-            if (MODE == RECOMPUTE) {
-              flush2(st + 2048, lane, p.out[1], p.ld_hi, row_base, p.M, g0, p.N);
-            } else if (p.a_hi != nullptr) {
-              flush2(st + 2048, lane, p.a_hi, p.ld_hi, row_base, p.M, g0, p.N);
-              flush2(st + 4096, lane, p.b_hi, p.ld_hi, row_base, p.M, g0, p.N);
-              flush1(st + 6144, lane, p.a_lo, p.ld_lo, row_base, p.M, g0, p.N);
-              flush1(st + 7168, lane, p.b_lo, p.ld_lo, row_base, p.M, g0, p.N);
+          for (int c = 0; c < CHUNKS; ++c) {
+            const int col0 = col_first + c * 16;
+            uint4 dh[2] = {};
+            if (MODE == RECOMPUTE && row < p.M) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                if (col0 + q * 8 < p.N) dh[q] = __ldg(reinterpret_cast<const uint4*>(p.dh + static_cast<size_t>(row) * p.ld_hi + col0 + q * 8));
             }
-            __syncwarp();
-          }
-        }
-      } else {
-        const bool fp32 = p.out_fp32[problem] != 0;
-        void* out = p.out[problem];
-#pragma unroll 1
-        for (int c = 0; c < TN / 16; ++c) {
-          const int col0 = n_blk * TN + c * 16;
-          uint32_t v[16];
-          tmem_ld_x16(t_row + c * 16, v);
-          tmem_ld_wait();
-          if (fp32) {
-            if (row < p.M) {
-              float* o = static_cast<float*>(out) + static_cast<size_t>(row) * p.ld_hi + col0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (col0 + q * 4 < p.N)
-                  reinterpret_cast<float4*>(o)[q] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]), __uint_as_float(v[4 * q + 2]),
-                                                               __uint_as_float(v[4 * q + 3]));
+            tmem_ld_wait();
+            if (c + 1 < CHUNKS) {
+              tmem_ld_x16(t_row + (c + 1) * 16, vg[(c + 1) & 1]);
+              tmem_ld_x16(t_row + TF + (c + 1) * 16, vu[(c + 1) & 1]);
             }
-          } else {
-            float f[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
-            put16(st, lane, (c & 1) * 2, f);
+            gated_chunk<MODE, ACT>(p, vg[c & 1], vu[c & 1], dh, col0, lane, st, (c & 1) * 2);
             if (c & 1) {
               __syncwarp();
-              flush2(st, lane, out, p.ld_hi, row_base, p.M, col0 - 16, p.N);
+              const int g0 = col0 - 16;
+              flush2(st, lane, p.out[0], p.ld_hi, row_base, p.M, g0, p.N);
+              if (MODE == RECOMPUTE) {
+                flush2(st + 2048, lane, p.out[1], p.ld_hi, row_base, p.M, g0, p.N);
+              } else if (p.a_hi != nullptr) {
+                flush2(st + 2048, lane, p.a_hi, p.ld_hi, row_base, p.M, g0, p.N);
+                flush2(st + 4096, lane, p.b_hi, p.ld_hi, row_base, p.M, g0, p.N);
+                flush1(st + 6144, lane, p.a_lo, p.ld_lo, row_base, p.M, g0, p.N);
+                flush1(st + 7168, lane, p.b_lo, p.ld_lo, row_base, p.M, g0, p.N);
+              }
               __syncwarp();
+            }
+          }
+        } else {
+          const bool fp32 = p.out_fp32[problem] != 0;
+          void* out = p.out[problem];
+          uint32_t v[2][16];
+          tmem_ld_x16(t_row, v[0]);
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) {
+            const int col0 = col_first + c * 16;
+            tmem_ld_wait();
+            if (c + 1 < CHUNKS) tmem_ld_x16(t_row + (c + 1) * 16, v[(c + 1) & 1]);
+            const uint32_t(&w)[16] = v[c & 1];
+            if (fp32) {
+              if (row < p.M) {
+                float* o = static_cast<float*>(out) + static_cast<size_t>(row) * p.ld_hi + col0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (col0 + q * 4 < p.N)
+                    reinterpret_cast<float4*>(o)[q] = make_float4(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1]), __uint_as_float(w[4 * q + 2]),
+                                                                 __uint_as_float(w[4 * q + 3]));
+              }
+            } else {
+              float f[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(w[i]);
+              put16(st, lane, (c & 1) * 2, f);
+              if (c & 1) {
+                __syncwarp();
+                flush2(st, lane, out, p.ld_hi, row_base, p.M, col0 - 16, p.N);
+                __syncwarp();
+              }
             }
           }
         }

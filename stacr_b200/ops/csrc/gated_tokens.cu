@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(WARPS * 32) gated_tokens_kernel(const Args a) 
     if (a.bg) gate += a.bg[f];
     if (a.bu) up += a.bu[f];
     float act, der;
-    act_and_derivative<ACT>(gate, act, der);
+    act_and_derivative<ACT, true>(gate, act, der);
     const size_t at = static_cast<size_t>(m) * a.F + f;
     a.h[at] = __float2bfloat16_rn(act * up);
     if (a.a_hi) {
