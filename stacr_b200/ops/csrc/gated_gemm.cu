@@ -25,6 +25,7 @@ namespace sb {
 int make_tensor_map_bf16(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer);
 
 namespace gt {
+bool takes(int M, int K, int F);
 int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,
             int act, cudaStream_t st);
 }
@@ -556,14 +557,14 @@ static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const 
 // h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) in bf16; x [M, K], weights [F, K] contiguous; K and F multiples of 8.
 // hi [2, M, F] 16-bit and lo [2, M, ceil16(F)] 8-bit receive the backward's factors; both null: not kept.
 extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, void* hi, void* lo, int M, int K, int F,
-                                int act, int tokens_max, int sms, int* status, void* stream) {
+                                int act, int sms, int* status, void* stream) {
   using namespace sb;
-  if (!gg::proper(M, K, F) || tokens_max > 64) return -2;
+  if (!gg::proper(M, K, F)) return -2;
   if (!gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(h) || !gg::aligned16(hi) || !gg::aligned16(lo)) return -3;
   const long long ld_lo = (F + 15) / 16 * 16;
   unsigned short* ah = static_cast<unsigned short*>(hi);
   unsigned char* al = static_cast<unsigned char*>(lo);
-  if (M <= tokens_max) return gt::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, static_cast<cudaStream_t>(stream));
+  if (gt::takes(M, K, F)) return gt::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, static_cast<cudaStream_t>(stream));
   gg::Params p{M, F, K, 1, {0, 0}, F, ld_lo, {h, nullptr}, {bg, bu}, nullptr, ah, ah ? ah + static_cast<size_t>(M) * F : nullptr, al, al ? al + M * ld_lo : nullptr,
                status};
   return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, static_cast<cudaStream_t>(stream));

@@ -1,12 +1,13 @@
 // Gated projections of a few tokens: h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) for M <= 64.
 //
-// Bound by the weights, 4 K F bytes that are read once; everything here serves that stream.  A CTA owns 16 features (16 rows of
+// Bound by the weights, 4 K F bytes that are read once (one token, K 4096, F 14336: 39.8 us, 5.9 TB/s, 0.90 of a copy's rate);
+// everything here serves that stream.  A CTA owns 16 features (16 rows of
 // each weight) and its eight warps share the reduction: warp w takes every eighth block of 32 values, so that the CTA reads 512
 // contiguous bytes of a row at a time.  Weights go from memory straight into the A fragments of mma.m16n8k16 (features are the
 // 16 rows, tokens the 8 columns): a reduction does not care which k sits where as long as both operands agree, so a thread's 16
 // contiguous bytes are its share of two instructions, and no shared memory, barrier or transpose stands between the
-// loads.  The tokens' B fragments are read the same way and hit L1 / L2.  At most 64 tokens keep the tensor work below the
-// stream's time on these instructions; tcgen05 would need its weights staged in shared memory and gains nothing here.
+// loads.  The tokens' B fragments are read the same way and hit L1 / L2.  Few tokens keep the tensor work far below
+// the stream's time on these instructions; tcgen05 would need its weights staged in shared memory and gains nothing here.
 // The eight partial sums meet in shared memory, in one order always.
 #include "gated.cuh"
 
@@ -40,7 +41,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 // NT: groups of 8 tokens.  U: blocks of 32 values whose weights are in flight together.
 template <int NT, int U, int ACT>
-__global__ void __launch_bounds__(WARPS * 32) gated_tokens_kernel(const Args a) {
+__global__ void __launch_bounds__(WARPS * 32, NT == 8 ? 1 : 2) gated_tokens_kernel(const Args a) {
   extern __shared__ float part[];                       // [WARPS][2][NT][FT * 8]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int f0 = blockIdx.x * FT;
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(WARPS * 32) gated_tokens_kernel(const Args a) 
   float cg[NT][4] = {}, cu[NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
   for (int k0 = warp * KB; k0 < a.K; k0 += WARPS * KB * U) {
-    uint4 v[U][4];
+    uint4 v[U][4], bx[U][NT];
 #pragma unroll
     for (int s = 0; s < U; ++s) {
       const int k = k0 + s * WARPS * KB + t * 8;
@@ -64,13 +65,19 @@ __global__ void __launch_bounds__(WARPS * 32) gated_tokens_kernel(const Args a) 
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int m = n * 8 + g;
-        const uint4 b = (m < a.M && k < a.K) ? __ldg(reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + k)) : zero;
+        bx[s][n] = (m < a.M && k < a.K) ? __ldg(reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + k)) : zero;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < U; ++s)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const uint4 b = bx[s][n];
         mma16816(cg[n], v[s][0].x, v[s][1].x, v[s][0].y, v[s][1].y, b.x, b.y);
         mma16816(cg[n], v[s][0].z, v[s][1].z, v[s][0].w, v[s][1].w, b.z, b.w);
         mma16816(cu[n], v[s][2].x, v[s][3].x, v[s][2].y, v[s][3].y, b.x, b.y);
         mma16816(cu[n], v[s][2].z, v[s][3].z, v[s][2].w, v[s][3].w, b.z, b.w);
       }
-    }
   }
   // partial sums, feature fastest: [warp][gate or up][token][feature]
   float* mine = part + warp * (2 * NT * FT * 8);
@@ -125,10 +132,19 @@ static int launch(const Args& a, cudaStream_t st) {
 
 template <int ACT>
 static int launch_tokens(const Args& a, cudaStream_t st) {
-  if (a.M <= 8) return launch<1, 2, ACT>(a, st);
-  if (a.M <= 16) return launch<2, 2, ACT>(a, st);
+  // as many blocks in flight as two CTAs per SM have registers for (one with 64 tokens)
+  if (a.M <= 8) return launch<1, 4, ACT>(a, st);
+  if (a.M <= 16) return launch<2, 3, ACT>(a, st);
   if (a.M <= 32) return launch<4, 2, ACT>(a, st);
   return launch<8, 2, ACT>(a, st);
+}
+
+// Whether this kernel is taken rather than the 256-token tiles, which read the weights at 6 TB/s but take 7 us for a single tile.
+// Measured per 16-feature pass (K 2048, F 8192, 67 MB): 8 tokens 12.0 us (5.6 TB/s), 16: 15.1, 32: 20.7, 64: 40.9; tiles 20; with
+// 4 MB (K 512, F 2048): 2.3, 2.7, 3.3, 4.7; tiles 9.  So up to 16 tokens always, and above while the weights are small.
+bool takes(int M, int K, int F) {
+  const double mb = 4e-6 * K * F;
+  return M <= 16 || (M <= 32 && mb <= 40) || (M <= 64 && mb <= 13);
 }
 
 int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,

@@ -9,9 +9,6 @@ from . import _lib
 from .nn_kernels import ACTIVATION_CODE
 
 
-TOKENS_MAX = 64     # up to this many tokens the forward pass streams the weights through csrc/gated_tokens.cu
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -26,8 +23,8 @@ def forward(x, wg, wu, bg, bu, activation: str, keep: bool):
     if keep:
         hi, lo = torch.empty((2, m, f), dtype=torch.int16, device=device), torch.empty((2, m, (f + 15) // 16 * 16), dtype=torch.uint8, device=device)
     sms, stream = _lib.place(x)
-    rc = _lib.entry("sb_gated_forward", "ppppppppiiiiiipp")(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), _ptr(hi), _ptr(lo), m, k, f,
-                                                         ACTIVATION_CODE[activation], TOKENS_MAX, sms, _lib.status_word(device).data_ptr(), stream)
+    rc = _lib.entry("sb_gated_forward", "ppppppppiiiiipp")(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), _ptr(hi), _ptr(lo), m, k, f,
+                                                         ACTIVATION_CODE[activation], sms, _lib.status_word(device).data_ptr(), stream)
     _lib.check_rc(rc, "sb_gated_forward")
     _lib.count(1)
     return h, ((hi, lo) if keep else None)
