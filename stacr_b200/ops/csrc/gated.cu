@@ -10,11 +10,6 @@
 
 namespace sb {
 
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-  T v[VEC];
-};
-
 struct GatedArgs {
   const void *gate, *up, *dout;
   void *out, *dgate, *dup;
@@ -30,24 +25,25 @@ __global__ void __launch_bounds__(256) gated_product_kernel(const GatedArgs a) {
     const P* u = reinterpret_cast<const P*>(static_cast<const T*>(a.up) + r * a.ld_up);
     const P* d = BWD ? reinterpret_cast<const P*>(static_cast<const T*>(a.dout) + r * a.ld_dout) : nullptr;
     for (long long c = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; c < nv; c += static_cast<long long>(gridDim.x) * blockDim.x) {
-      const P gv = g[c], uv = u[c];
-      P o1, o2;
+      float gv[VEC], uv[VEC], o1[VEC];
+      unpack(g[c], gv);
+      unpack(u[c], uv);
       if (BWD) {
-        const P dv = d[c];
+        float dv[VEC], o2[VEC];
+        unpack(d[c], dv);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float act, der;
-          act_and_derivative<ACT, false>(to_f32(gv.v[i]), act, der);
-          const float dd = to_f32(dv.v[i]);
-          o1.v[i] = from_f32<T>(dd * to_f32(uv.v[i]) * der);
-          o2.v[i] = from_f32<T>(dd * act);
+          act_and_derivative<ACT, sizeof(T) == 2>(gv[i], act, der);
+          o1[i] = dv[i] * uv[i] * der;
+          o2[i] = dv[i] * act;
         }
-        if (a.dgate) reinterpret_cast<P*>(static_cast<T*>(a.dgate) + r * a.n)[c] = o1;
-        if (a.dup) reinterpret_cast<P*>(static_cast<T*>(a.dup) + r * a.n)[c] = o2;
+        if (a.dgate) reinterpret_cast<P*>(static_cast<T*>(a.dgate) + r * a.n)[c] = pack<T, VEC>(o1);
+        if (a.dup) reinterpret_cast<P*>(static_cast<T*>(a.dup) + r * a.n)[c] = pack<T, VEC>(o2);
       } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o1.v[i] = from_f32<T>(activation<ACT>(to_f32(gv.v[i])) * to_f32(uv.v[i]));
-        reinterpret_cast<P*>(static_cast<T*>(a.out) + r * a.n)[c] = o1;
+        for (int i = 0; i < VEC; ++i) o1[i] = activation<ACT, sizeof(T) == 2>(gv[i]) * uv[i];
+        reinterpret_cast<P*>(static_cast<T*>(a.out) + r * a.n)[c] = pack<T, VEC>(o1);
       }
     }
   }

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace sb {
@@ -21,6 +23,32 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// VEC neighbouring values as one access, and to and from fp32 (16-bit types two at a time).
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&f)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) f[i] = to_f32(p.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC]) {
+  Pack<T, VEC> p;
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(p.v)[i / 2] = __floats2half2_rn(f[i], f[i + 1]);
+      else reinterpret_cast<__nv_bfloat162*>(p.v)[i / 2] = __floats2bfloat162_rn(f[i], f[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p.v[i] = from_f32<T>(f[i]);
+  }
+  return p;
+}
+
 // e^x as 2^t (1 + r ln 2) with t = fl(x log2 e) and r the rounding error of that product, which one fma recovers: the library
 // is compiled for fast math, whose exponential drops r and is off by |x| 2^-24.  Infinite t is left alone (r would be NaN).
 __device__ __forceinline__ float exp_f32(float x) {
@@ -32,7 +60,7 @@ __device__ __forceinline__ float exp_f32(float x) {
 }
 
 // 1 / (1 + e^-x).  e^-x overflows to infinity below x = -88, where the result is 0.  FAST: the hardware's exponential and reciprocal,
-// off by (3 + 1.2 |x|) 2^-23 of the result: for results that are rounded to bf16 (2^-8) or kept in 24 bits (2^-16).
+// off by (3 + 1.2 |x|) 2^-23 of the result: for results that are rounded to 16-bit types (fp16: 2^-11) or kept in 24 bits (2^-16).
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_f32(float x) {
   return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : __frcp_rn(1.f + exp_f32(-x));
@@ -64,10 +92,10 @@ __device__ __forceinline__ unsigned upper24(float v) {
   return (b & 0x7fffffffu) < 0x7f800000u ? b + 0x80u : b;
 }
 
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float activation(float x) {
   float act, der;
-  act_and_derivative<ACT, false>(x, act, der);
+  act_and_derivative<ACT, FAST>(x, act, der);
   return act;
 }
 

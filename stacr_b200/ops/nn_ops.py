@@ -581,7 +581,8 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
     inv = inv_freq
     if inv.dtype != torch.float64 or inv.device != q.device or inv.requires_grad or not inv.is_contiguous():
         inv = inv.detach().to(device=q.device, dtype=torch.float64).contiguous()
-    if q.is_cuda and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and q.numel() + (0 if k is None else k.numel()) > 0 and _lib.available():
+    if (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and d <= 1024
+            and q.numel() + (0 if k is None else k.numel()) > 0 and _lib.available()):
         if positions is not None and positions.dtype not in (torch.int32, torch.int64):
             positions = positions.to(torch.int64)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
