@@ -193,7 +193,7 @@ _ENTRIES: dict = {}
 _LETTERS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
 
 
-def entry(name: str, letters: str):
+def entry(name: str, letters: str, result: str = "i"):
     """An entry point with declared argument types (one letter each: pointer, int, long long, float, double).
 
     Plain Python numbers then convert by themselves, which costs a launch several microseconds less than wrapping each in a
@@ -202,7 +202,7 @@ def entry(name: str, letters: str):
     fn = _ENTRIES.get(name)
     if fn is None:
         fn = getattr(load(), name)
-        fn.argtypes, fn.restype = [_LETTERS[c] for c in letters], ctypes.c_int
+        fn.argtypes, fn.restype = [_LETTERS[c] for c in letters], _LETTERS[result]
         _ENTRIES[name] = fn
     return fn
 

@@ -2,7 +2,7 @@
 //
 //   forward       G = x Wg^T + bg,  U = x Wu^T + bu,  h = act(G) U       one kernel, G and U exist in tensor memory only
 //   recomputing   the same G and U again, and from them and dh:  dG = dh U act'(G),  dU = dh act(G)
-//   input grad    dx = dG Wg + dU Wu                                     one accumulator over both products
+//   input grad    dx = dG Wg + dU Wu                                     one accumulator over both products, see share()
 //   weight grads  dWg = dG^T x,  dWu = dU^T x                            one launch over the tiles of both
 //
 // Forward and recomputation work on tiles of 256 tokens x 128 features.  Each CTA stages its own 128 tokens of x; the even CTA
@@ -58,7 +58,19 @@ struct Params {
   unsigned short *a_hi, *b_hi;   // kept factors, null: not kept
   unsigned char *a_lo, *b_lo;
   int* status;
+  int whole, splits;        // INPUT_GRAD, WEIGHT_GRAD: tiles [0, whole) are reduced by one pair each, the others in `splits` parts
+  float4* partial;          // one 256 x 256 fp32 tile a part, [part][64 groups of 4 columns][256 rows]
 };
+
+// What a pair does at a time: a tile, and the k-blocks of its reduction.  A part of a split tile leaves its fp32 sums in slot `part`.
+struct Unit {
+  int tile, kb0, kb1, part;
+};
+__device__ __forceinline__ Unit unit_at(const Params& p, int u, int num_kb) {
+  if (u < p.whole) return {u, 0, num_kb, -1};
+  const int v = u - p.whole, tile = v / p.splits, k = v - tile * p.splits, per = (num_kb + p.splits - 1) / p.splits;
+  return {p.whole + tile, k * per, (k + 1) * per < num_kb ? (k + 1) * per : num_kb, v};
+}
 
 __device__ __forceinline__ void decode(int tile, int num_m, int num_n, int& m_blk, int& n_blk) {
   constexpr int G = 4;       // rows of tiles that run side by side: their x and weight tiles are shared through L2
@@ -195,6 +207,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
   const int num_kb = MODE == INPUT_GRAD ? 2 * kb_one : kb_one;       // both products fall into one accumulator
   const int tiles_one = num_m * num_n;
   const int total_tiles = MODE == WEIGHT_GRAD ? tiles_one * p.problems : tiles_one;
+  const int total_units = p.whole + (total_tiles - p.whole) * p.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -224,13 +237,14 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int tile = pair; tile < total_tiles && ok; tile += npairs) {
-        const int problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
+      for (int u = pair; u < total_units && ok; u += npairs) {
+        const Unit unit = unit_at(p, u, num_kb);
+        const int tile = unit.tile, problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
         int m_blk, n_blk;
         decode(tile - problem * tiles_one, num_m, num_n, m_blk, n_blk);
         const int m0 = m_blk * TM + static_cast<int>(crank) * HM;
         const int n0 = PROJECT ? n_blk * TF : n_blk * TN + static_cast<int>(crank) * HM;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = unit.kb0; kb < unit.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, p.status, ST_TIMEOUT_SMEM_EMPTY)) {
             ok = false;
             break;
@@ -269,7 +283,8 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
       uint32_t ph = 0;
       int local = 0;
       bool ok = true;
-      for (int tile = pair; tile < total_tiles && ok; tile += npairs, ++local) {
+      for (int u = pair; u < total_units && ok; u += npairs, ++local) {
+        const Unit unit = unit_at(p, u, num_kb);
         const int acc = local & 1;
         const uint32_t acc_ph = (local >> 1) & 1;
         if (!mbar_wait(&tmem_empty[acc], acc_ph ^ 1u, abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY)) {
@@ -278,7 +293,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * TN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = unit.kb0; kb < unit.kb1; ++kb) {
           if (!mbar_wait(&full_bar[s], ph, abort_flag, p.status, ST_TIMEOUT_SMEM_FULL)) {
             ok = false;
             break;
@@ -290,7 +305,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
           for (int j = 0; j < BK / UMMA_K; ++j) {
             const uint64_t adesc = A_MN ? make_smem_desc_sw128(sa + j * 2048, 8192, 1024) : make_smem_desc_sw128(sa + j * 32, 16, 1024);
             const uint64_t bdesc = B_MN ? make_smem_desc_sw128(sb_ + j * 2048, 8192, 1024) : make_smem_desc_sw128(sb_ + j * 32, 16, 1024);
-            umma_bf16_pair(d_tmem, adesc, bdesc, idesc, (kb > 0 || j > 0) ? 1u : 0u);
+            umma_bf16_pair(d_tmem, adesc, bdesc, idesc, (kb > unit.kb0 || j > 0) ? 1u : 0u);
           }
           umma_commit_pair(&empty_bar[s]);
           if (++s == STAGES) {
@@ -307,8 +322,9 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
     uint8_t* st = epi_stage + (warp - 2) * WARP_EPI;
     int local = 0;
     bool ok = true;
-    for (int tile = pair; tile < total_tiles && ok; tile += npairs, ++local) {
-      const int problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
+    for (int u = pair; u < total_units && ok; u += npairs, ++local) {
+      const Unit unit = unit_at(p, u, num_kb);
+      const int tile = unit.tile, problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
       int m_blk, n_blk;
       decode(tile - problem * tiles_one, num_m, num_n, m_blk, n_blk);
       const int acc = local & 1;
@@ -371,7 +387,12 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
             tmem_ld_wait();
             if (c + 1 < CHUNKS) tmem_ld_x16(t_row + (c + 1) * 16, v[(c + 1) & 1]);
             const uint32_t(&w)[16] = v[c & 1];
-            if (fp32) {
+            if (unit.part >= 0) {       // neighbouring lanes are neighbouring rows: whole lines
+              float4* part = p.partial + (static_cast<size_t>(unit.part) * 64 + (half * CHUNKS + c) * 4) * TM + static_cast<int>(crank) * HM + quad * 32 + lane;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                part[q * TM] = make_float4(__uint_as_float(w[4 * q]), __uint_as_float(w[4 * q + 1]), __uint_as_float(w[4 * q + 2]), __uint_as_float(w[4 * q + 3]));
+            } else if (fp32) {
               if (row < p.M) {
                 float* o = static_cast<float*>(out) + static_cast<size_t>(row) * p.ld_hi + col0;
 #pragma unroll
@@ -415,6 +436,66 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
   }
 }
 
+// Sums of the parts of the split tiles, in the order of the parts.  A block has 16 columns of a tile, a thread one row of them.
+template <int MODE>
+__global__ void __launch_bounds__(TM) gated_join_kernel(const __grid_constant__ Params p) {
+  const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + TN - 1) / TN, tiles_one = num_m * num_n;
+  const int split_tile = blockIdx.x >> 4, c = blockIdx.x & 15;
+  const int tile = p.whole + split_tile, problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
+  int m_blk, n_blk;
+  decode(tile - problem * tiles_one, num_m, num_n, m_blk, n_blk);
+  const int row = m_blk * TM + threadIdx.x, col0 = n_blk * TN + c * 16;
+  if (row >= p.M || col0 >= p.N) return;
+  float f[16] = {};
+  const float4* part = p.partial + (static_cast<size_t>(split_tile) * p.splits * 64 + c * 4) * TM + threadIdx.x;
+  for (int k = 0; k < p.splits; ++k, part += 64 * TM)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 v = part[q * TM];
+      f[4 * q] += v.x, f[4 * q + 1] += v.y, f[4 * q + 2] += v.z, f[4 * q + 3] += v.w;
+    }
+  const size_t at = static_cast<size_t>(row) * p.ld_hi + col0;
+  if (p.out_fp32[problem]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col0 + q * 4 < p.N) reinterpret_cast<float4*>(static_cast<float*>(p.out[problem]) + at)[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (col0 + q * 8 < p.N)
+        reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out[problem]) + at)[q] =
+            make_uint4(pack_bf16x2(f[8 * q], f[8 * q + 1]), pack_bf16x2(f[8 * q + 2], f[8 * q + 3]), pack_bf16x2(f[8 * q + 4], f[8 * q + 5]),
+                       pack_bf16x2(f[8 * q + 6], f[8 * q + 7]));
+  }
+}
+
+// How the reductions of `tiles` tiles of num_kb k-blocks are shared among the pairs.  Tiles are dealt out in rounds; the last
+// round, or the only one, rarely has a tile for every pair, and the idle ones take parts of its reductions instead.  Joining the
+// parts costs a second kernel of about 4 us, 14 k-blocks' time (0.28 us each), so a split has to shorten the round by more: 24.
+// 512 tokens of K 2048, F 8192: dx has 16 tiles for 74 pairs, 103 us whole, 51 in four parts; 8192 tokens: 3.5 rounds of tiles
+// instead of four.
+struct Shares {
+  int whole, splits;
+};
+static Shares share(long long tiles, int num_kb, int sms) {
+  const int pairs = sms / 2 < 1 ? 1 : sms / 2;
+  const int last = static_cast<int>(tiles % pairs);
+  if (last == 0) return {static_cast<int>(tiles), 1};
+  int splits = pairs / last;
+  if (splits > num_kb / 8) splits = num_kb / 8;
+  if (splits < 2) return {static_cast<int>(tiles), 1};
+  const int per = (num_kb + splits - 1) / splits;
+  splits = (num_kb + per - 1) / per;        // no part is empty
+  if (num_kb - per < 24) return {static_cast<int>(tiles), 1};
+  return {static_cast<int>(tiles) - last, splits};
+}
+static long long tiles_of(int rows, int cols) { return static_cast<long long>((rows + TM - 1) / TM) * ((cols + TN - 1) / TN); }
+static int blocks_of(int k) { return (k + BK - 1) / BK; }
+static size_t partial_bytes(long long tiles, int num_kb, int sms) {
+  const Shares s = share(tiles, num_kb, sms);
+  return static_cast<size_t>(tiles - s.whole) * s.splits * TM * TN * 4;
+}
+
 template <int MODE, int ACT>
 static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMap& b0, const CUtensorMap& b1, const Params& p, int sms, cudaStream_t stream) {
   static PerDeviceOnce once;
@@ -429,8 +510,9 @@ static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMa
   constexpr int STEP_N = MODE <= RECOMPUTE ? TF : TN;
   const long long tiles = static_cast<long long>((p.M + TM - 1) / TM) * ((p.N + STEP_N - 1) / STEP_N) * (MODE == WEIGHT_GRAD ? p.problems : 1);
   if (tiles > 0x3fffffff) return -2;
+  const long long units = p.whole + (tiles - p.whole) * p.splits;
   int pairs = sms / 2;
-  if (pairs > tiles) pairs = static_cast<int>(tiles);
+  if (pairs > units) pairs = static_cast<int>(units);
   if (pairs < 1) pairs = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs, 1, 1);
@@ -444,7 +526,15 @@ static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMa
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, p));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, p);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if constexpr (MODE == INPUT_GRAD || MODE == WEIGHT_GRAD) {
+    if (tiles > p.whole) {
+      gated_join_kernel<MODE><<<static_cast<unsigned>((tiles - p.whole) * 16), TM, 0, stream>>>(p);
+      return static_cast<int>(cudaGetLastError());
+    }
+  }
+  return 0;
 }
 
 template <int MODE>
@@ -496,6 +586,8 @@ static bool proper(int M, int K, int F) { return M > 0 && K > 0 && F > 0 && K % 
 
 template <int MODE>
 static int project(const void* x, const void* wg, const void* wu, Params& p, int act, int sms, cudaStream_t st) {
+  p.whole = static_cast<int>(static_cast<long long>((p.M + TM - 1) / TM) * ((p.N + TF - 1) / TF));
+  p.splits = 1;
   CUtensorMap ta, tg, tu;
   int rc = make_tensor_map_bf16(&ta, x, p.K, p.M, p.K, HM);
   if (!rc) rc = make_tensor_map_bf16(&tg, wg, p.K, p.N, p.K, HM);
@@ -522,20 +614,21 @@ static int factors(const void* dh, const unsigned short* hi, const unsigned char
 
 // dx[M, K] = dG Wg + dU Wu
 static int input_grad(const __nv_bfloat16* dg, const __nv_bfloat16* du, const void* wg, const void* wu, void* dx, int M, int K, int F, int sms, int* status,
-                      cudaStream_t st) {
+                      float4* partial, cudaStream_t st) {
   CUtensorMap a0, a1, b0, b1;
   int rc = make_tensor_map_bf16(&a0, dg, F, M, F, HM);
   if (!rc) rc = make_tensor_map_bf16(&a1, du, F, M, F, HM);
   if (!rc) rc = make_tensor_map_bf16(&b0, wg, K, F, K, 64);
   if (!rc) rc = make_tensor_map_bf16(&b1, wu, K, F, K, 64);
   if (rc) return rc;
-  Params p{M, K, F, 1, {0, 0}, K, 0, {dx, nullptr}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
+  const Shares sh = share(tiles_of(M, K), 2 * blocks_of(F), sms);
+  Params p{M, K, F, 1, {0, 0}, K, 0, {dx, nullptr}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status, sh.whole, sh.splits, partial};
   return launch<INPUT_GRAD, ACT_SILU>(a0, a1, b0, b1, p, sms, st);
 }
 
 // dWg = dG^T x and dWu = dU^T x [F, K], each fp32 or bf16; a null result is left out
 static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const void* x, void* dwg, void* dwu, int fp32_g, int fp32_u, int M, int K, int F,
-                        int sms, int* status, cudaStream_t st) {
+                        int sms, int* status, float4* partial, cudaStream_t st) {
   if (!dwg) {
     dg = du;
     dwg = dwu;
@@ -547,7 +640,9 @@ static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const 
   if (!rc) rc = make_tensor_map_bf16(&a1, dwu ? du : dg, F, M, F, 64);
   if (!rc) rc = make_tensor_map_bf16(&b, x, K, M, K, 64);
   if (rc) return rc;
-  Params p{F, K, M, dwu ? 2 : 1, {fp32_g, fp32_u}, K, 0, {dwg, dwu}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status};
+  const Shares sh = share(tiles_of(F, K) * (dwu ? 2 : 1), blocks_of(M), sms);
+  Params p{F, K, M, dwu ? 2 : 1, {fp32_g, fp32_u}, K, 0, {dwg, dwu}, {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, nullptr, status, sh.whole, sh.splits,
+           partial};
   return launch<WEIGHT_GRAD, ACT_SILU>(a0, a1, b, b, p, sms, st);
 }
 
@@ -570,15 +665,27 @@ extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, c
   return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, static_cast<cudaStream_t>(stream));
 }
 
+// Bytes that `partial` of sb_gated_backward has to hold; 0: it may be null.
+extern "C" long long sb_gated_partial_bytes(int M, int K, int F, int need_dx, int weights, int sms) {
+  using namespace sb::gg;
+  if (!proper(M, K, F)) return 0;
+  size_t most = need_dx ? partial_bytes(tiles_of(M, K), 2 * blocks_of(F), sms) : 0;
+  if (weights > 0) {
+    const size_t w = partial_bytes(tiles_of(F, K) * weights, blocks_of(M), sms);
+    if (w > most) most = w;
+  }
+  return static_cast<long long>(most);
+}
+
 // d [2, M, F] = dG and dU, from the kept factors or (hi null) from the projections formed again; dx [M, K] unless null; the weight
 // gradients [F, K], each fp32 or bf16, unless null.
 extern "C" int sb_gated_backward(const void* dh, const void* x, const void* wg, const void* wu, const float* bg, const float* bu, const void* hi, const void* lo,
-                                 void* d, void* dx, void* dwg, void* dwu, int fp32_g, int fp32_u, int M, int K, int F, int act, int sms, int* status,
-                                 void* stream) {
+                                 void* d, void* dx, void* dwg, void* dwu, void* partial, long long partial_size, int fp32_g, int fp32_u, int M, int K, int F,
+                                 int act, int sms, int* status, void* stream) {
   using namespace sb;
-  if (!gg::proper(M, K, F)) return -2;
+  if (!gg::proper(M, K, F) || partial_size < sb_gated_partial_bytes(M, K, F, dx != nullptr, (dwg != nullptr) + (dwu != nullptr), sms)) return -2;
   if (!gg::aligned16(dh) || !gg::aligned16(x) || !gg::aligned16(wg) || !gg::aligned16(wu) || !gg::aligned16(hi) || !gg::aligned16(lo) || !gg::aligned16(d) ||
-      !gg::aligned16(dx) || !gg::aligned16(dwg) || !gg::aligned16(dwu))
+      !gg::aligned16(dx) || !gg::aligned16(dwg) || !gg::aligned16(dwu) || !gg::aligned16(partial))
     return -3;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   __nv_bfloat16* dg = static_cast<__nv_bfloat16*>(d);
@@ -590,7 +697,7 @@ extern "C" int sb_gated_backward(const void* dh, const void* x, const void* wg, 
     gg::Params p{M, F, K, 1, {0, 0}, F, 0, {dg, du}, {bg, bu}, static_cast<const __nv_bfloat16*>(dh), nullptr, nullptr, nullptr, nullptr, status};
     rc = gg::project<gg::RECOMPUTE>(x, wg, wu, p, act, sms, st);
   }
-  if (!rc && dx) rc = gg::input_grad(dg, du, wg, wu, dx, M, K, F, sms, status, st);
-  if (!rc && (dwg || dwu)) rc = gg::weight_grads(dg, du, x, dwg, dwu, fp32_g, fp32_u, M, K, F, sms, status, st);
+  if (!rc && dx) rc = gg::input_grad(dg, du, wg, wu, dx, M, K, F, sms, status, static_cast<float4*>(partial), st);
+  if (!rc && (dwg || dwu)) rc = gg::weight_grads(dg, du, x, dwg, dwu, fp32_g, fp32_u, M, K, F, sms, status, static_cast<float4*>(partial), st);
   return rc;
 }

@@ -40,9 +40,11 @@ def backward(dh, x, wg, wu, bg, bu, activation: str, kept, need_dx: bool, out_ga
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=device) if need_dx else None
     hi, lo = kept if kept is not None else (None, None)
     sms, stream = _lib.place(x)
-    rc = _lib.entry("sb_gated_backward", "pppppppppppp" + "iiiiiii" + "pp")(
+    size = _lib.entry("sb_gated_partial_bytes", "iiiiii", "l")(m, k, f, need_dx, int(out_gate is not None) + int(out_up is not None), sms)
+    partial = torch.empty(size, dtype=torch.uint8, device=device) if size else None       # sums of split reductions
+    rc = _lib.entry("sb_gated_backward", "pppppppppppp" + "pl" + "iiiiiii" + "pp")(
         dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), _ptr(bg), _ptr(bu), _ptr(hi), _ptr(lo), d.data_ptr(), _ptr(dx), _ptr(out_gate), _ptr(out_up),
-        out_gate is not None and out_gate.dtype == torch.float32, out_up is not None and out_up.dtype == torch.float32, m, k, f, ACTIVATION_CODE[activation], sms,
+        _ptr(partial), size, out_gate is not None and out_gate.dtype == torch.float32, out_up is not None and out_up.dtype == torch.float32, m, k, f, ACTIVATION_CODE[activation], sms,
         _lib.status_word(device).data_ptr(), stream)
     _lib.check_rc(rc, "sb_gated_backward")
     _lib.count(1 + int(need_dx) + int(out_gate is not None or out_up is not None))

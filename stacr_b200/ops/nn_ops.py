@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
-from . import _lib
+from . import _lib, gated, nn_kernels
 
 
 def _kernel_tensor(x: torch.Tensor) -> bool:
@@ -523,8 +523,6 @@ class _RotaryFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, inv_freq, positions, first, interleaved, scale):
-        from . import nn_kernels
-
         ctx.save_for_backward(inv_freq, positions)
         ctx.set_materialize_grads(False)
         ctx.first, ctx.interleaved, ctx.scale = first, interleaved, scale
@@ -534,8 +532,6 @@ class _RotaryFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        from . import nn_kernels
-
         inv_freq, positions = ctx.saved_tensors
         gq = _heads(gq) if ctx.needs_input_grad[0] else None
         gk = _heads(gk) if ctx.needs_input_grad[1] else None
@@ -587,8 +583,6 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
             positions = positions.to(torch.int64)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             return _RotaryFn.apply(q, k, inv, positions, first, bool(interleaved), float(scale))
-        from . import nn_kernels
-
         with _lib.on_device(q):
             return nn_kernels.rotary(_heads(q), _heads(k), inv, positions, first, bool(interleaved), float(scale), 1.0)
     where = torch.arange(first, first + s, device=q.device)[None] if positions is None else positions
@@ -624,8 +618,6 @@ def _flat_rows(*ts: torch.Tensor):
 
 
 def _gated_product(gate, up, activation):
-    from . import nn_kernels
-
     with _lib.on_device(gate):
         g2, u2 = _flat_rows(_rows(gate), _rows(up))
         return nn_kernels.gated_product_fwd(g2, u2, activation).view(gate.shape)
@@ -641,8 +633,6 @@ class _GatedProductFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        from . import nn_kernels
-
         gate, up = ctx.saved_tensors
         with _lib.on_device(gate):
             d2, g2, u2 = _flat_rows(_rows(dout), _rows(gate), _rows(up))
@@ -671,8 +661,8 @@ def gated_product(gate, up, activation: str = "silu"):
 def _take_slot(weight):
     """The fp32 buffer a gradient synchroniser has lent for this weight's gradient, or ``None``."""
     slot = getattr(weight, "_sb_grad_out", None) if getattr(weight, "_sb_grad_fresh", False) else None
-    if slot is None or slot.dtype != torch.float32 or weight.dtype != torch.float32:
-        return None
+    if slot is None or slot.dtype != torch.float32 or weight.dtype != torch.float32 or not slot.is_contiguous() or slot.data_ptr() % 16:
+        return None         # the gradient then goes back through autograd, which adds it to the slot
     weight._sb_grad_fresh = False
     return slot
 
@@ -686,12 +676,24 @@ def _hand_over(weight, dw, slot):
     return dw if dw.dtype == weight.dtype else dw.to(weight.dtype)
 
 
+def _operand(t):
+    """``t`` as the tensor-core kernels read it: bf16, contiguous and on a 16-byte boundary (a copy where it is not)."""
+    t = (t if t.dtype == torch.bfloat16 else t.detach().to(torch.bfloat16)).contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _bf16_operand(weight):
-    if weight.dtype == torch.bfloat16 and weight.is_contiguous():
-        return weight
+    if weight.dtype == torch.bfloat16:
+        return _operand(weight)
     from ..layers import _bf16_weight
 
-    return _bf16_weight(weight).contiguous()
+    return _operand(_bf16_weight(weight))
+
+
+def _weight_gradient_buffer(weight, slot):
+    """Where a weight's gradient is formed: the lent slot, else a new matrix, fp32 unless the weight itself is bf16."""
+    return slot if slot is not None else torch.empty(weight.shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32,
+                                                     device=weight.device)
 
 
 class _GatedLinearFn(torch.autograd.Function):
@@ -703,10 +705,8 @@ class _GatedLinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2d, gate_weight, up_weight, gate_bias, up_bias, activation, recompute):
-        from . import gated
-
         with _lib.on_device(x2d):
-            xa = (x2d if x2d.dtype == torch.bfloat16 else x2d.to(torch.bfloat16)).contiguous()
+            xa = _operand(x2d)
             h, kept = gated.forward(xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), activation,
                                     keep=not recompute)
         ctx.save_for_backward(xa, gate_weight, up_weight, gate_bias, up_bias, *(kept or ()))
@@ -716,26 +716,31 @@ class _GatedLinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        from . import gated, stacr_ops
-
         xa, gate_weight, up_weight, gate_bias, up_bias, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dbg = dbu = None
         with _lib.on_device(xa):
-            dh = (dh if dh.dtype == torch.bfloat16 else dh.to(torch.bfloat16)).contiguous()
+            dh = _operand(dh)
             same = gate_weight is up_weight       # one weight in both places receives two gradients: neither may use its slot
-            slots = [None if same or not need[i + 1] else _take_slot(w) for i, w in enumerate((gate_weight, up_weight))]
-            dw = [None if not need[i + 1] else slots[i] if slots[i] is not None else
-                  torch.empty(w.shape, dtype=torch.bfloat16 if w.dtype == torch.bfloat16 else torch.float32, device=w.device)
-                  for i, w in enumerate((gate_weight, up_weight))]
+            gslot = _take_slot(gate_weight) if need[1] and not same else None
+            uslot = _take_slot(up_weight) if need[2] and not same else None
+            dwg = _weight_gradient_buffer(gate_weight, gslot) if need[1] else None
+            dwu = _weight_gradient_buffer(up_weight, uslot) if need[2] else None
             d, dx = gated.backward(dh, xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), ctx.activation,
-                                   kept or None, need[0], *dw)
+                                   kept or None, need[0], dwg, dwu)
             if dx is not None and dx.dtype != ctx.in_dtype:
                 dx = dx.to(ctx.in_dtype)
-            dwg, dwu = (None if g is None else _hand_over(w, g, slot) for w, g, slot in zip((gate_weight, up_weight), dw, slots))
+            if dwg is not None:
+                dwg = _hand_over(gate_weight, dwg, gslot)
+            if dwu is not None:
+                dwu = _hand_over(up_weight, dwu, uslot)
             if gate_bias is not None and need[3]:
+                from . import stacr_ops
+
                 dbg = stacr_ops.colsum(d[0]).to(gate_bias.dtype)
             if up_bias is not None and need[4]:
+                from . import stacr_ops
+
                 dbu = stacr_ops.colsum(d[1]).to(up_bias.dtype)
         return dx, dwg, dwu, dbg, dbu, None, None
 
@@ -771,9 +776,7 @@ def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, act
                                     or any(b is not None and b.requires_grad for b in (gate_bias, up_bias))):
         h = _GatedLinearFn.apply(x2d, gate_weight, up_weight, gate_bias, up_bias, activation, bool(recompute))
     else:
-        from . import gated
-
         with _lib.on_device(x):
-            h = gated.forward((x2d if x2d.dtype == torch.bfloat16 else x2d.detach().to(torch.bfloat16)).contiguous(), _bf16_operand(gate_weight), _bf16_operand(up_weight),
-                              _f32_bias(gate_bias), _f32_bias(up_bias), activation, keep=False)[0]
+            h = gated.forward(_operand(x2d), _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), activation,
+                              keep=False)[0]
     return h if x.dim() == 2 else h.reshape(*x.shape[:-1], gate_weight.shape[0])

@@ -249,7 +249,7 @@ def gated_inputs(m, k, f, seed=0, dtype=torch.bfloat16):
 
 
 GATED_SHAPES = [(1, 8, 8), (1, 2048, 688), (2, 64, 136), (7, 1000, 264), (17, 512, 1000), (33, 1536, 896), (64, 72, 128), (65, 200, 2056), (127, 256, 688),
-                (129, 512, 520), (254, 256, 688), (257, 1032, 384), (1000, 264, 1096), (1531, 768, 2048)]
+                (129, 512, 520), (254, 256, 688), (257, 1032, 384), (1000, 264, 1096), (1531, 768, 2048), (4100, 264, 520), (5000, 72, 136)]
 
 
 @pytest.mark.parametrize("recompute", [False, True])
@@ -342,6 +342,27 @@ def test_gated_linear_uses_lent_gradient_slots():
     for p, w in zip(lent, want):
         assert torch.equal(p._sb_grad_out, w)
     assert bool((flat[:32] == 7).all() and (flat[-32:] == 7).all())
+
+
+@pytest.mark.parametrize("m", [3, 70])
+def test_gated_linear_takes_operands_of_any_alignment_and_order(m):
+    from stacr_b200.ops import nn_ops
+
+    tensors = [t for i, t in enumerate(gated_inputs(m, 64, 136)) if i not in (3, 4)]
+    want = None
+    for move in ("as is", "shifted", "transposed"):
+        moved = []
+        for t in tensors:
+            if move == "shifted":       # two bytes behind a 16-byte boundary
+                t = torch.cat((t.new_zeros(1), t.reshape(-1)))[1:].view(t.shape)
+            elif move == "transposed":
+                t = t.t().contiguous().t()
+            moved.append(t)
+        leaves = [t.detach().requires_grad_() for t in moved[:3]]
+        h = nn_ops.gated_linear(*leaves)
+        got = [h.detach(), *torch.autograd.grad(h, leaves, moved[3])]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), move
 
 
 def test_gated_linear_nonfinite_values_stay_in_their_rows_and_columns():
