@@ -53,6 +53,12 @@ def is_plain_linear(module: nn.Module) -> bool:
         module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
+def saved_tensors_are_hooked() -> bool:
+    """Whether saved-tensor hooks are installed: a compressor, an offloader or a checkpoint that works on what autograd saves."""
+    top = getattr(torch._C._autograd, "_top_saved_tensors_default_hooks", None)
+    return top is not None and top(False) is not None
+
+
 class Embedding(nn.Embedding):
     """``nn.Embedding`` (same parameter, same state-dict key) whose bf16-autocast path on a B200 is the in-tree lookup and
     scatter-add (see ``ops.nn_ops.embedding``); the output is then already in the autocast dtype."""

@@ -7,9 +7,10 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.nn import functional as F
 
 from ..ops import nn_ops
-from .common import causal_attention, Embedding, init_weights, is_plain_linear, Linear, lm_loss, ModelOutput
+from .common import causal_attention, Embedding, init_weights, is_plain_linear, Linear, lm_loss, ModelOutput, saved_tensors_are_hooked
 from .neox import apply_rotary, rotary_tables
 
 
@@ -105,6 +106,8 @@ class LlamaMLP(nn.Module):
 
     def forward(self, x):
         gate, up = self.gate_proj, self.up_proj
+        if saved_tensors_are_hooked():      # the hooks get the activations that separate layers save, in their own type
+            return self.down_proj(F.silu(gate(x)) * up(x))
         if is_plain_linear(gate) and is_plain_linear(up) and nn_ops.gated_linear_supported(x, gate.weight, up.weight):
             h = nn_ops.gated_linear(x, gate.weight, up.weight, gate.bias, up.bias, recompute=self.recompute)
         else:                       # compressed or adapted projections, other devices and types

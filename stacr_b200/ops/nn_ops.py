@@ -549,7 +549,7 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
     """Rotary positions: ``(q', k')`` for ``q`` ``[B, S, heads, D]`` and ``k`` ``[B, S, kv_heads, D]`` (or ``None``).
 
     ``inv_freq`` (see :func:`rotary_frequencies`) has ``rot / 2`` angular frequencies; the first ``rot <= D`` values of a head are
-    turned, as pairs ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)``, and the rest is copied.  Pair ``i`` at position ``p`` is
+    turned (``inv_freq`` itself receives no gradient), as pairs ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)``, and the rest is copied.  Pair ``i`` at position ``p`` is
     turned by ``p * inv_freq[i]`` and multiplied by ``scale``; the angle is formed in 64 bits.  ``positions`` is ``None`` (``0 .. S-1``),
     an int (the first token's position), or an integer tensor ``[S]``, ``[1, S]``, ``[B, 1]`` or ``[B, S]``.  Inputs may have any strides
     (a transposed ``[B, heads, S, D]`` view is read in place); results are contiguous.
@@ -557,28 +557,34 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("rotary expects q and k as [batch, sequence, heads, head_dim]")
     b, s, _, d = q.shape
-    if k is not None and (k.shape[0] != b or k.shape[1] != s or k.shape[3] != d):
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, sequence or head_dim")
-    if k is not None and (k.dtype != q.dtype or k.device != q.device):
-        raise ValueError("q and k must have one dtype and one device")
-    if not q.is_floating_point():
-        raise TypeError(f"rotary expects floating-point heads, got {q.dtype}")
-    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 0 < 2 * inv_freq.numel() <= d:
+    dtype = q.dtype
+    if k is not None:
+        kb, ks, _, kd = k.shape
+        if kb != b or ks != s or kd != d:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, sequence or head_dim")
+        if k.dtype is not dtype or k.device != q.device:
+            raise ValueError("q and k must have one dtype and one device")
+    if not dtype.is_floating_point:
+        raise TypeError(f"rotary expects floating-point heads, got {dtype}")
+    if inv_freq.dim() != 1 or not inv_freq.dtype.is_floating_point or not 0 < 2 * inv_freq.numel() <= d:
         raise ValueError(f"inv_freq must hold 1 to {d // 2} frequencies, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
     first = 0
     if isinstance(positions, int):
         first, positions = positions, None
     elif positions is not None:
-        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
-            raise TypeError(f"positions must be integers, got {positions.dtype}")
-        if positions.dim() not in (1, 2) or positions.shape[-1] not in (1, s) or (positions.dim() == 2 and positions.shape[0] not in (1, b)):
-            raise ValueError(f"positions {tuple(positions.shape)} do not fit [{b}, {s}]")
-        positions = (positions if positions.device == q.device else positions.to(q.device)).expand(b, s)
+        kind, shape = positions.dtype, tuple(positions.shape)
+        if kind.is_floating_point or kind.is_complex or kind is torch.bool:
+            raise TypeError(f"positions must be integers, got {kind}")
+        if shape != (b, s):
+            if len(shape) not in (1, 2) or shape[-1] not in (1, s) or (len(shape) == 2 and shape[0] not in (1, b)):
+                raise ValueError(f"positions {shape} do not fit [{b}, {s}]")
+            positions = positions.expand(b, s)
+        if positions.device != q.device:
+            positions = positions.to(q.device)
     inv = inv_freq
-    if inv.dtype != torch.float64 or inv.device != q.device or inv.requires_grad or not inv.is_contiguous():
+    if inv.dtype is not torch.float64 or inv.device != q.device or inv.requires_grad or not inv.is_contiguous():
         inv = inv.detach().to(device=q.device, dtype=torch.float64).contiguous()
-    if (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16, torch.float32) and d <= 1024
-            and q.numel() + (0 if k is None else k.numel()) > 0 and _lib.available()):
+    if q.is_cuda and dtype in nn_kernels.DTYPE_CODE and d <= 1024 and (q.numel() or (k is not None and k.numel())):
         if positions is not None and positions.dtype not in (torch.int32, torch.int64):
             positions = positions.to(torch.int64)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -649,8 +655,7 @@ def gated_product(gate, up, activation: str = "silu"):
     _check_activation(activation)
     if gate.shape != up.shape:
         raise ValueError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} differ in shape")
-    if (gate.is_cuda and gate.device == up.device and gate.dtype == up.dtype and gate.dtype in (torch.bfloat16, torch.float16, torch.float32)
-            and gate.numel() > 0 and gate.dim() > 0 and _lib.available()):
+    if gate.is_cuda and gate.dtype is up.dtype and gate.dtype in nn_kernels.DTYPE_CODE and gate.device == up.device and gate.numel() and gate.dim():
         if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
             return _GatedProductFn.apply(gate, up, activation)
         return _gated_product(gate, up, activation)
@@ -751,9 +756,11 @@ def _f32_bias(bias):
 
 def gated_linear_supported(x, gate_weight, up_weight) -> bool:
     """Whether :func:`gated_linear` takes its kernels for these operands (bf16 activations, or bf16 autocast, on one GPU)."""
-    return (x.is_cuda and x.device == gate_weight.device == up_weight.device and gate_weight.dim() == 2 and x.shape[-1] % 8 == 0
-            and gate_weight.shape[0] % 8 == 0 and x.numel() > 0 and gate_weight.numel() > 0 and _lib.available()
-            and (x.dtype == torch.bfloat16 or (torch.is_autocast_enabled() and torch.get_autocast_dtype("cuda") == torch.bfloat16)))
+    if not x.is_cuda or gate_weight.dim() != 2:
+        return False
+    f, k = gate_weight.shape
+    return (f % 8 == 0 and k % 8 == 0 and f > 0 and x.numel() > 0 and x.device == gate_weight.device == up_weight.device
+            and (x.dtype is torch.bfloat16 or (torch.is_autocast_enabled() and torch.get_autocast_dtype("cuda") == torch.bfloat16)))
 
 
 def gated_linear(x, gate_weight, up_weight, gate_bias=None, up_bias=None, *, activation: str = "silu", recompute: bool = False):

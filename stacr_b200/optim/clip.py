@@ -77,21 +77,21 @@ def grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor]) -> torch.Tensor
 
 
 def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """Scale all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and return their norm from before, as a device scalar.
 
     The call of ``torch.nn.utils.clip_grad_norm_``.  Dense bf16, fp16 and fp32 gradients on one GPU take the kernels, which sum the
     2-norm beyond fp32's range and decide about the scaling on the device, so the host does not wait (``error_if_nonfinite``
     does, and raises before anything is scaled) and the call can be captured into a CUDA graph.  A gradient that occurs
     twice counts and is scaled once; gradients that overlap in part are refused.  Everything else (other norms, other layouts or
-    devices, sharded tensors) goes to the framework's function.
+    devices, sharded tensors) goes to the framework's function, with ``foreach``.
     """
     max_norm, norm_type = float(max_norm), float(norm_type)
     params = _parameters(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     table = _kernel_table(grads) if norm_type == 2.0 else None
     if table is None:
-        return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite)
+        return torch.nn.utils.clip_grad_norm_(params, max_norm, norm_type, error_if_nonfinite, foreach)
     if error_if_nonfinite:
         norm = _run(grads, table, None)
         if not bool(torch.isfinite(norm)):

@@ -50,6 +50,13 @@ def test_rotary_positions_forms_agree():
     assert torch.equal(nn_ops.rotary(q, None, inv, torch.tensor([[4], [9]]))[0][1], nn_ops.rotary(q[1:], None, inv, torch.full((1, 3), 9))[0][0])
 
 
+def test_rotary_of_nothing():
+    inv, _ = nn_ops.rotary_frequencies(8)
+    for shape in ((0, 3, 2, 8), (2, 0, 2, 8), (2, 3, 0, 8)):
+        q, k = nn_ops.rotary(torch.zeros(shape), torch.zeros(shape), inv)
+        assert q.shape == k.shape == shape
+
+
 def test_rotary_refusals():
     inv, _ = nn_ops.rotary_frequencies(8)
     q, k = torch.randn(2, 3, 4, 8), torch.randn(2, 3, 2, 8)

@@ -401,6 +401,37 @@ def test_gated_linear_repeats_bit_for_bit_and_runs_on_a_side_stream():
     assert torch.equal(runs[0][0], runs[2][0])
 
 
+@pytest.mark.parametrize("recompute", [False, True])
+def test_gated_linear_offsets_beyond_32_bits(recompute):
+    from stacr_b200.ops import nn_ops
+
+    m, k, f = 270001, 64, 8192          # 2.2e9 features
+    x, wg, wu, bg, bu, _ = gated_inputs(m, k, f)
+    dh = torch.randn(1, f, device="cuda").bfloat16().expand(m, f)
+    xl = x.requires_grad_()
+    h = nn_ops.gated_linear(xl, wg, wu, bg, bu, recompute=recompute)
+    (dx,) = torch.autograd.grad(h, xl, dh)
+    for rows in (slice(0, 40), slice(262140, 262180), slice(m - 40, m)):
+        leaves = (x.detach()[rows], wg, wu, bg, bu)
+        g, u, want, grads = gated_exact(*leaves, dh[rows], "silu")
+        bounds = gated_bounds(*leaves, dh[rows], "silu", g, u, keep=not recompute)
+        inside(h.detach()[rows], want, bounds[0], "h")
+        inside(dx[rows], grads[0], bounds[1], "dx")
+
+
+def test_gated_product_sizes_beyond_32_bits():
+    from stacr_b200.ops import nn_ops
+
+    n = 2 ** 31 + 9
+    gate = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    gate[-5:] = 2.0
+    gate[:3] = 1.0
+    out = nn_ops.gated_product(gate, gate)
+    want = F.silu(torch.tensor([1.0, 2.0], dtype=torch.float64)) * torch.tensor([1.0, 2.0], dtype=torch.float64)
+    assert bool((out[:3] == want[0].to(torch.bfloat16).cuda()).all()) and bool((out[-5:] == want[1].to(torch.bfloat16).cuda()).all())
+    assert not bool(out[3:-5].any())
+
+
 # ------------------------------------------------------------------------------------------------ gradient norm and clipping
 def clip_params(shapes, dtypes, std=1.0, seed=0):
     gen = torch.Generator(device="cuda").manual_seed(seed)
@@ -570,6 +601,20 @@ def test_llama_step_with_the_fused_block_tracks_fp32(recompute):
     assert abs(float(norm) - float(total)) <= (16 / 2 + 2) * 2.0 ** -24 * float(total)
     after = torch.stack([p.grad.double().square().sum() for p in model.parameters()]).sum().sqrt()
     assert abs(float(after) - 0.1) < 1e-6
+
+
+def test_llama_under_saved_tensor_hooks_saves_what_separate_layers_save():
+    from stacr_b200.models import build_model
+
+    torch.manual_seed(0)
+    model = build_model("llama-tiny").cuda()
+    ids = torch.randint(0, 1024, (1, 40), device="cuda")
+    saved = []
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t) or t, lambda t: t):
+        model(input_ids=ids, labels=ids).loss.backward()
+    assert not any(t.dtype in (torch.int16, torch.uint8) for t in saved)
+    # gate, its activation and up in each of the two layers, and the down projection's input
+    assert sum(t.dtype == torch.bfloat16 and t.shape[-1] == 688 and t.numel() == 40 * 688 for t in saved) >= 8
 
 
 def test_llama_step_replayed_from_a_cuda_graph_equals_the_eager_step():
