@@ -25,9 +25,12 @@ namespace sb {
 int make_tensor_map_bf16(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer);
 
 namespace gt {
-bool takes(int M, int K, int F);
 int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,
             int act, cudaStream_t st);
+}
+namespace gf {
+int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,
+            int act, int sms, int* status, cudaStream_t st);
 }
 
 namespace gg {
@@ -649,6 +652,26 @@ static int weight_grads(const __nv_bfloat16* dg, const __nv_bfloat16* du, const 
 }  // namespace gg
 }  // namespace sb
 
+namespace sb {
+namespace gg {
+
+// Which forward kernel: for at most 128 tokens one that streams the weights, whichever of the two the following lines, fitted to
+// measurements at weights of 0.7 to 272 MB, expect to be done first; above, the 256-token tiles of this file.
+//   gated_tokens.cu (to 64 tokens): 2 us and the weights at 6, 4.9, 3.2 and 1.7 TB/s for 8, 16, 32 and 64 tokens.  Measured at
+//     67 MB (K 2048, F 8192): 12.5, 15.3, 20.6, 40.8 us, at 4 MB (K 512, F 2048): 2.3, 2.7, 3.3, 4.7.
+//   gated_few.cu: 4.4 us and 0.27 for each k-block, or 3.5 and the weights at 5.9 TB/s, and more for more columns to finish.
+//     Measured at the same: 15.1, 15.4, 15.9, 15.8 us (128 tokens: 17.9); 5.9, 5.9, 6.0, 6.7 (8.3).
+//   tiles, 128 tokens: 19.8 and 9.3.
+static bool streams_fragments(int M, int K, int F) {
+  if (M > 64) return false;
+  const double mb = 4e-6 * K * F, chain = 4.4 + 0.27 * (K / 64.0), stream = 3.5 + mb / 5.9;
+  const double tokens = 2.0 + mb / (M <= 8 ? 6.0 : M <= 16 ? 4.9 : M <= 32 ? 3.2 : 1.7);
+  return tokens <= (chain > stream ? chain : stream) + (M > 32 ? 0.8 : 0.0);
+}
+
+}  // namespace gg
+}  // namespace sb
+
 // h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) in bf16; x [M, K], weights [F, K] contiguous; K and F multiples of 8.
 // hi [2, M, F] 16-bit and lo [2, M, ceil16(F)] 8-bit receive the backward's factors; both null: not kept.
 extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, void* hi, void* lo, int M, int K, int F,
@@ -659,10 +682,12 @@ extern "C" int sb_gated_forward(const void* x, const void* wg, const void* wu, c
   const long long ld_lo = (F + 15) / 16 * 16;
   unsigned short* ah = static_cast<unsigned short*>(hi);
   unsigned char* al = static_cast<unsigned char*>(lo);
-  if (gt::takes(M, K, F)) return gt::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (gg::streams_fragments(M, K, F)) return gt::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, st);
+  if (M <= 128) return gf::forward(x, wg, wu, bg, bu, h, ah, al, M, K, F, act, sms, status, st);
   gg::Params p{M, F, K, 1, {0, 0}, F, ld_lo, {h, nullptr}, {bg, bu}, nullptr, ah, ah ? ah + static_cast<size_t>(M) * F : nullptr, al, al ? al + M * ld_lo : nullptr,
                status};
-  return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, static_cast<cudaStream_t>(stream));
+  return gg::project<gg::FORWARD>(x, wg, wu, p, act, sms, st);
 }
 
 // Bytes that `partial` of sb_gated_backward has to hold; 0: it may be null.

@@ -1,4 +1,4 @@
-// Gated projections of a few tokens: h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) for M <= 64.
+// Gated projections of single tokens: h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) for M <= 64 (see sb_gated_forward for when).
 //
 // Bound by the weights, 4 K F bytes that are read once (one token, K 4096, F 14336: 39.8 us, 5.9 TB/s, 0.90 of a copy's rate);
 // everything here serves that stream.  A CTA owns 16 features (16 rows of
@@ -137,14 +137,6 @@ static int launch_tokens(const Args& a, cudaStream_t st) {
   if (a.M <= 16) return launch<2, 3, ACT>(a, st);
   if (a.M <= 32) return launch<4, 2, ACT>(a, st);
   return launch<8, 2, ACT>(a, st);
-}
-
-// Whether this kernel is taken rather than the 256-token tiles, which read the weights at 6 TB/s but take 7 us for a single tile.
-// Measured per 16-feature pass (K 2048, F 8192, 67 MB): 8 tokens 12.0 us (5.6 TB/s), 16: 15.1, 32: 20.7, 64: 40.9; tiles 20; with
-// 4 MB (K 512, F 2048): 2.3, 2.7, 3.3, 4.7; tiles 9.  So up to 16 tokens always, and above while the weights are small.
-bool takes(int M, int K, int F) {
-  const double mb = 4e-6 * K * F;
-  return M <= 16 || (M <= 32 && mb <= 40) || (M <= 64 && mb <= 13);
 }
 
 int forward(const void* x, const void* wg, const void* wu, const float* bg, const float* bu, void* h, unsigned short* hi, unsigned char* lo, int M, int K, int F,

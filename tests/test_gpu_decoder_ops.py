@@ -249,7 +249,9 @@ def gated_inputs(m, k, f, seed=0, dtype=torch.bfloat16):
 
 
 GATED_SHAPES = [(1, 8, 8), (1, 2048, 688), (2, 64, 136), (7, 1000, 264), (17, 512, 1000), (33, 1536, 896), (64, 72, 128), (65, 200, 2056), (127, 256, 688),
-                (129, 512, 520), (254, 256, 688), (257, 1032, 384), (1000, 264, 1096), (1531, 768, 2048), (4100, 264, 520), (5000, 72, 136)]
+                (129, 512, 520), (254, 256, 688), (257, 1032, 384), (1000, 264, 1096), (1531, 768, 2048), (4100, 264, 520), (5000, 72, 136),
+                # each token count of the kernel for some tokens, with whole and ragged features
+                (16, 1024, 16384), (13, 1032, 16392), (32, 256, 14336), (27, 264, 14344), (64, 256, 14336), (50, 264, 14344), (128, 64, 256)]
 
 
 @pytest.mark.parametrize("recompute", [False, True])
