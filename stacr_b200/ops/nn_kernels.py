@@ -181,13 +181,42 @@ DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 ACTIVATION_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 
+def _row_stride(t: torch.Tensor):
+    """Elements from one row (last dimension) of ``t`` to the next, or ``None`` where the rows do not lie at equal steps."""
+    sizes, strides = t.shape, t.stride()
+    if sizes[-1] != 1 and strides[-1] != 1:
+        return None
+    step, expected = None, None
+    for size, stride in zip(reversed(sizes[:-1]), reversed(strides[:-1])):
+        if size == 1:
+            continue
+        if step is None:
+            step = stride
+        elif stride != expected:
+            return None
+        expected = stride * size
+    return 0 if step is None else step
+
+
+def _as_rows(*ts: torch.Tensor):
+    """``(tensors, rows, n, row strides)``: contiguous tensors as one row, so that a width that is no multiple of a vector costs only the
+    last few elements; others as rows where they lie at equal steps, and copied where they do not."""
+    if all(t.is_contiguous() for t in ts):
+        return ts, 1, ts[0].numel(), (0,) * len(ts)
+    steps = [_row_stride(t) for t in ts]
+    if None in steps:
+        ts = tuple(t if s is not None else t.contiguous() for t, s in zip(ts, steps))
+        steps = [_row_stride(t) for t in ts]
+    n = ts[0].shape[-1]
+    return ts, ts[0].numel() // n, n, steps
+
+
 def gated_product_fwd(gate: torch.Tensor, up: torch.Tensor, activation: str) -> torch.Tensor:
-    """``act(gate) * up`` of two ``[rows, n]`` matrices with contiguous columns; the result is contiguous."""
-    rows, n = gate.shape
+    """``act(gate) * up`` of two tensors of one shape; the result is contiguous."""
+    (gate, up), rows, n, (lg, lu) = _as_rows(gate, up)
     out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
     rc = _lib.entry("sb_gated_product_fwd", "pppllll" + "iiip")(
-        gate.data_ptr(), up.data_ptr(), out.data_ptr(), gate.stride(0), up.stride(0), rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation],
-        *_lib.place(gate))
+        gate.data_ptr(), up.data_ptr(), out.data_ptr(), lg, lu, rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation], *_lib.place(gate))
     _lib.check_rc(rc, "sb_gated_product_fwd")
     _lib.count(1)
     return out
@@ -195,12 +224,12 @@ def gated_product_fwd(gate: torch.Tensor, up: torch.Tensor, activation: str) -> 
 
 def gated_product_bwd(dout: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, activation: str, need_gate: bool = True, need_up: bool = True):
     """``(dgate, dup)`` of :func:`gated_product_fwd`, contiguous; ``None`` for one that is not needed."""
-    rows, n = gate.shape
+    (dout, gate, up), rows, n, (ld, lg, lu) = _as_rows(dout, gate, up)
     dgate = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device) if need_gate else None
     dup = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device) if need_up else None
     rc = _lib.entry("sb_gated_product_bwd", "ppppplllll" + "iiip")(
-        dout.data_ptr(), gate.data_ptr(), up.data_ptr(), None if dgate is None else dgate.data_ptr(), None if dup is None else dup.data_ptr(), dout.stride(0),
-        gate.stride(0), up.stride(0), rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation], *_lib.place(gate))
+        dout.data_ptr(), gate.data_ptr(), up.data_ptr(), None if dgate is None else dgate.data_ptr(), None if dup is None else dup.data_ptr(), ld, lg, lu,
+        rows, n, DTYPE_CODE[gate.dtype], ACTIVATION_CODE[activation], *_lib.place(gate))
     _lib.check_rc(rc, "sb_gated_product_bwd")
     _lib.count(1)
     return dgate, dup

@@ -21,6 +21,16 @@ def _kernel_tensor(x: torch.Tensor) -> bool:
     return x.is_cuda and x.dtype == torch.bfloat16
 
 
+def _differentiable_once(backward):
+    """``once_differentiable`` for a backward of kernels: its wrapper is entered only where a graph of the backward is being recorded."""
+    recorded = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
+
+
 # ------------------------------------------------------------------------------ LayerNorm
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
@@ -530,7 +540,7 @@ class _RotaryFn(torch.autograd.Function):
             return nn_kernels.rotary(_heads(q), _heads(k), inv_freq, positions, first, interleaved, scale, 1.0)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, gq, gk):
         inv_freq, positions = ctx.saved_tensors
         gq = _heads(gq) if ctx.needs_input_grad[0] else None
@@ -605,45 +615,22 @@ def _check_activation(activation: str) -> None:
         raise ValueError(f"unknown activation {activation!r}; choose from {sorted(_ACTIVATIONS)}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as a matrix with contiguous columns: a view where its strides allow one, else a copy."""
-    n = t.shape[-1]
-    if t.stride(-1) == 1 or n == 1:
-        try:
-            return t.view(-1, n) if t.dim() != 2 else t
-        except RuntimeError:
-            pass
-    return t.reshape(-1, n).contiguous()
-
-
-def _flat_rows(*ts: torch.Tensor):
-    """The matrices as one row when all are contiguous: widths that are no multiple of a vector then cost only the last few elements."""
-    if all(t.is_contiguous() for t in ts):
-        return tuple(t.view(1, -1) for t in ts)
-    return ts
-
-
-def _gated_product(gate, up, activation):
-    with _lib.on_device(gate):
-        g2, u2 = _flat_rows(_rows(gate), _rows(up))
-        return nn_kernels.gated_product_fwd(g2, u2, activation).view(gate.shape)
-
-
 class _GatedProductFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, activation):
         ctx.save_for_backward(gate, up)
         ctx.activation = activation
-        return _gated_product(gate, up, activation)
+        with _lib.on_device(gate):
+            return nn_kernels.gated_product_fwd(gate, up, activation)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dout):
         gate, up = ctx.saved_tensors
+        need_gate, need_up, _ = ctx.needs_input_grad
         with _lib.on_device(gate):
-            d2, g2, u2 = _flat_rows(_rows(dout), _rows(gate), _rows(up))
-            dgate, dup = nn_kernels.gated_product_bwd(d2, g2, u2, ctx.activation, *ctx.needs_input_grad[:2])
-        return None if dgate is None else dgate.view(gate.shape), None if dup is None else dup.view(up.shape), None
+            dgate, dup = nn_kernels.gated_product_bwd(dout, gate, up, ctx.activation, need_gate, need_up)
+        return dgate, dup, None
 
 
 def gated_product(gate, up, activation: str = "silu"):
@@ -658,7 +645,8 @@ def gated_product(gate, up, activation: str = "silu"):
     if gate.is_cuda and gate.dtype is up.dtype and gate.dtype in nn_kernels.DTYPE_CODE and gate.device == up.device and gate.numel() and gate.dim():
         if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
             return _GatedProductFn.apply(gate, up, activation)
-        return _gated_product(gate, up, activation)
+        with _lib.on_device(gate):
+            return nn_kernels.gated_product_fwd(gate, up, activation)
     return _ACTIVATIONS[activation](gate) * up
 
 
@@ -719,7 +707,7 @@ class _GatedLinearFn(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dh):
         xa, gate_weight, up_weight, gate_bias, up_bias, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
