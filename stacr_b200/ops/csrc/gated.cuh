@@ -49,6 +49,17 @@ __device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC]) {
   return p;
 }
 
+// Inputs and results of the kernels never overlap, so loads may pass stores: the non-coherent path says so to the compiler.
+template <typename P>
+__device__ __forceinline__ P load_once(const void* p) {
+  P v;
+  if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = __ldg(static_cast<const uint4*>(p));
+  else if constexpr (sizeof(P) == 8) *reinterpret_cast<uint2*>(&v) = __ldg(static_cast<const uint2*>(p));
+  else if constexpr (sizeof(P) == 4) *reinterpret_cast<unsigned*>(&v) = __ldg(static_cast<const unsigned*>(p));
+  else *reinterpret_cast<unsigned short*>(&v) = __ldg(static_cast<const unsigned short*>(p));
+  return v;
+}
+
 // e^x as 2^t (1 + r ln 2) with t = fl(x log2 e) and r the rounding error of that product, which one fma recovers: the library
 // is compiled for fast math, whose exponential drops r and is off by |x| 2^-24.  Infinite t is left alone (r would be NaN).
 __device__ __forceinline__ float exp_f32(float x) {
@@ -72,11 +83,18 @@ __device__ __forceinline__ float sigmoid_f32(float x) {
 //   gelu_tanh  x s,        s (1 + x (1 - s) 2 w'),          s = sigmoid(2 w) = (1 + tanh w) / 2,  w = sqrt(2/pi) (x + 0.044715 x^3)
 template <int ACT, bool FAST>
 __device__ __forceinline__ void act_and_derivative(float x, float& act, float& der) {
-  if (ACT == ACT_GELU) {
-    const float cdf = FAST ? 0.5f + 0.5f * erff(0.707106781f * x) : 0.5f * erfcf(-0.707106781f * x);
-    const float pdf = 0.398942280f * (FAST ? __expf(-0.5f * x * x) : exp_f32(-0.5f * x * x));
+  if (ACT == ACT_GELU && FAST) {
+    // Abramowitz and Stegun 7.1.26, erfc(z) = (a1 t + ... + a5 t^5) e^-z^2 with t = 1 / (1 + p z), off by at most 1.5e-7; the
+    // exponential is the density's too (8192 x 8192 values in bf16: 76 us forward and 114 backward, 93 and 131 with erff)
+    const float e = __expf(-0.5f * x * x), t = __fdividef(1.f, fmaf(0.3275911f * 0.707106781f, fabsf(x), 1.f));
+    const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float cdf = x < 0.f ? tail : 1.f - tail;
     act = x * cdf;
-    der = fmaf(x, pdf, cdf);
+    der = fmaf(x, 0.398942280f * e, cdf);
+  } else if (ACT == ACT_GELU) {
+    const float cdf = 0.5f * erfcf(-0.707106781f * x);
+    act = x * cdf;
+    der = fmaf(x, 0.398942280f * exp_f32(-0.5f * x * x), cdf);
   } else {
     const float k = 1.59576912f, c = 0.044715f;   // 2 sqrt(2/pi)
     const float s = sigmoid_f32<FAST>(ACT == ACT_SILU ? x : k * x * fmaf(c * x, x, 1.f));

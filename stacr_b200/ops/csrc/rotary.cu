@@ -42,17 +42,6 @@ struct RotaryArgs {
 constexpr int ROT_THREADS = 320;   // threads of a block at most
 constexpr int ROT_TOKENS = 4;      // tokens of a block
 
-// Inputs and results never overlap, so loads may pass stores: the non-coherent path says so to the compiler.
-template <typename P>
-__device__ __forceinline__ P load_once(const void* p) {
-  P v;
-  if constexpr (sizeof(P) == 16) *reinterpret_cast<uint4*>(&v) = __ldg(static_cast<const uint4*>(p));
-  else if constexpr (sizeof(P) == 8) *reinterpret_cast<uint2*>(&v) = __ldg(static_cast<const uint2*>(p));
-  else if constexpr (sizeof(P) == 4) *reinterpret_cast<unsigned*>(&v) = __ldg(static_cast<const unsigned*>(p));
-  else *reinterpret_cast<unsigned short*>(&v) = __ldg(static_cast<const unsigned short*>(p));
-  return v;
-}
-
 template <typename T, int VEC, bool INTER, bool MIXED>
 __global__ void __launch_bounds__(VEC == 1 ? 1024 : ROT_THREADS, VEC == 1 ? 1 : 4) rotary_kernel(const RotaryArgs a, int heads_side, int tokens_most) {
   using P = Pack<T, VEC>;
