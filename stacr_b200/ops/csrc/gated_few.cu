@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
     const float* bias_of = is_gate ? a.bg : a.bu;
     const float bias = bias_of != nullptr && f < a.F ? bias_of[f] : 0.f;
     // when every product is done every copy has landed and been read: the stages' memory is free
-    const bool ok = mbar_wait(done_bar, 0, abort_flag, a.status, ST_TIMEOUT_TMEM_FULL);
+    // (the whole warp goes on or gives up together: the tensor memory loads are warp-wide instructions)
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, a.status, ST_TIMEOUT_TMEM_FULL));
     tc_fence_after();
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     float* trade = reinterpret_cast<float*>(smem) + fl;   // [token][feature]: up of the first half of the tokens, gate of the second

@@ -336,7 +336,8 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
       const int row = row_base + lane;
       constexpr int CHUNKS = (PROJECT ? TF : TN) / 32;            // chunks of 16 columns in this warp's half
       const int col_first = n_blk * STEP_N + half * CHUNKS * 16;
-      if (!mbar_wait(&tmem_full[acc], acc_ph, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL)) {
+      // the whole warp goes on or gives up together: the tensor memory loads below are warp-wide instructions
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_ph, abort_flag, p.status, ST_TIMEOUT_TMEM_FULL))) {
         ok = false;
         break;
       }

@@ -43,7 +43,7 @@ constexpr int ROT_THREADS = 320;   // threads of a block at most
 constexpr int ROT_TOKENS = 4;      // tokens of a block
 
 template <typename T, int VEC, bool INTER, bool MIXED>
-__global__ void __launch_bounds__(VEC == 1 ? 1024 : ROT_THREADS, VEC == 1 ? 1 : 4) rotary_kernel(const RotaryArgs a, int heads_side, int tokens_most) {
+__global__ void __launch_bounds__(VEC == 1 ? 512 : ROT_THREADS, VEC == 1 ? 2 : 4) rotary_kernel(const RotaryArgs a, int heads_side, int tokens_most) {
   using P = Pack<T, VEC>;
   constexpr bool SINGLE = INTER && VEC > 1;                              // both values of a pair lie in one vector
   constexpr int PAIRS = MIXED ? VEC : SINGLE ? VEC / 2 : INTER ? 1 : VEC;   // sines of a turning slot; MIXED: one for each value
@@ -168,7 +168,7 @@ template <typename T, int VEC, bool INTER, bool MIXED>
 static int rotary_launch(const RotaryArgs& a, int sms, cudaStream_t st) {
   const int turning = MIXED ? (a.rot + VEC - 1) / VEC : INTER ? a.rot / (VEC > 1 ? VEC : 2) : (a.rot / 2) / VEC;
   const int copied = MIXED ? a.D / VEC - turning : (a.D - a.rot) / VEC, slots = turning + copied;
-  const int heads = a.hq + a.hk, most = VEC == 1 ? 1024 : ROT_THREADS;
+  const int heads = a.hq + a.hk, most = VEC == 1 ? 512 : ROT_THREADS;
   if (slots > most) return -2;
   // as many heads as the block has threads for, evened out over the blocks that takes
   const int rounds = (heads + most / slots - 1) / (most / slots), side = (heads + rounds - 1) / rounds;
@@ -215,14 +215,14 @@ static int rotary_typed(const RotaryArgs& a, int sms, cudaStream_t st) {
 }  // namespace sb
 
 // q [B, S, hq, D] and k [B, S, hk, D] (null with hk = 0) with the strides given, into contiguous oq, ok; dtype 0 bf16, 1 fp16, 2 fp32.
-// rot is even, 2 <= rot <= D.  sign +1 forward, -1 backward.
+// rot is even, 2 <= rot <= D <= 512 (a head's vectors are the threads of one block).  sign +1 forward, -1 backward.
 extern "C" int sb_rotary(const void* q, const void* k, void* oq, void* ok, long long qb, long long qs, long long qh, long long kb, long long ks, long long kh,
                          const double* inv_freq, const void* positions, int pos64, long long pb, long long ps, long long first, long long B, int S, int hq,
                          int hk, int D, int rot, int interleaved, int dtype, float scale, float sign, int sms, void* stream) {
   using namespace sb;
   using namespace sb::rot;
   if (B <= 0 || S <= 0 || hq + hk <= 0) return 0;
-  if (rot < 2 || rot % 2 || rot > D || D > 1024 || hq < 0 || hk < 0) return -2;
+  if (rot < 2 || rot % 2 || rot > D || D > 512 || hq < 0 || hk < 0) return -2;
   RotaryArgs a{q, k, oq, ok, qb, qs, qh, kb, ks, kh, inv_freq, positions, pb, ps, first, B, S, hq, hk, D, rot, pos64, 1, scale, sign};
   if (S == 1 && B <= 0x7fffffffLL) {     // one token a sequence: the batch takes the sequence's place, all at the first position
     a.qs = qb, a.ks = kb, a.ps = pb;

@@ -594,7 +594,7 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
     inv = inv_freq
     if inv.dtype is not torch.float64 or inv.device != q.device or inv.requires_grad or not inv.is_contiguous():
         inv = inv.detach().to(device=q.device, dtype=torch.float64).contiguous()
-    if q.is_cuda and dtype in nn_kernels.DTYPE_CODE and d <= 1024 and (q.numel() or (k is not None and k.numel())):
+    if q.is_cuda and dtype in nn_kernels.DTYPE_CODE and d <= 512 and (q.numel() or (k is not None and k.numel())):
         if positions is not None and positions.dtype not in (torch.int32, torch.int64):
             positions = positions.to(torch.int64)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -655,7 +655,7 @@ def _take_slot(weight):
     """The fp32 buffer a gradient synchroniser has lent for this weight's gradient, or ``None``."""
     slot = getattr(weight, "_sb_grad_out", None) if getattr(weight, "_sb_grad_fresh", False) else None
     if slot is None or slot.dtype != torch.float32 or weight.dtype != torch.float32 or not slot.is_contiguous() or slot.data_ptr() % 16:
-        return None         # the gradient then goes back through autograd, which adds it to the slot
+        return None         # the gradient then goes back through autograd, and the synchroniser moves it
     weight._sb_grad_fresh = False
     return slot
 

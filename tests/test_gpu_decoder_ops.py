@@ -48,7 +48,8 @@ def rotary_bound(x, positions, inv, interleaved, scale):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("b,s,hq,hk,d,rot", [(1, 1, 1, 1, 2, 2), (3, 7, 4, 2, 64, 64), (2, 65, 28, 4, 128, 128), (1, 130, 5, 5, 80, 20), (2, 9, 3, 1, 30, 6),
-                                             (64, 1, 32, 8, 64, 64), (1, 2049, 2, 1, 96, 48)])
+                                             (64, 1, 32, 8, 64, 64), (1, 2049, 2, 1, 96, 48),
+                                             (2, 5, 1, 1, 512, 510), (1, 3, 2, 1, 509, 506), (1, 2, 1, 1, 520, 520), (1, 3000, 71, 1, 16, 8)])
 def test_rotary_forward_and_backward(b, s, hq, hk, d, rot, interleaved, dtype):
     from stacr_b200.ops import nn_ops
 
@@ -107,6 +108,17 @@ def test_rotary_positions_types_offsets_and_partial_gradients():
     with pytest.raises(RuntimeError):
         (g,) = torch.autograd.grad(nn_ops.rotary(q, None, inv)[0].sum(), q, create_graph=True)
         g.sum().backward()
+
+
+def test_gated_operators_refuse_second_derivatives():
+    from stacr_b200.ops import nn_ops
+
+    x, wg, wu, _, _, _ = gated_inputs(9, 16, 24)
+    for call in (lambda t: nn_ops.gated_product(t, t), lambda t: nn_ops.gated_linear(t, wg, wu)):
+        leaf = x.detach().clone().requires_grad_()
+        (g,) = torch.autograd.grad(call(leaf).float().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.float().sum().backward()
 
 
 def test_rotary_offsets_beyond_32_bits():
@@ -432,6 +444,45 @@ def test_gated_product_sizes_beyond_32_bits():
     want = F.silu(torch.tensor([1.0, 2.0], dtype=torch.float64)) * torch.tensor([1.0, 2.0], dtype=torch.float64)
     assert bool((out[:3] == want[0].to(torch.bfloat16).cuda()).all()) and bool((out[-5:] == want[1].to(torch.bfloat16).cuda()).all())
     assert not bool(out[3:-5].any())
+
+
+def test_two_captured_graphs_replayed_at_once_do_not_disturb_each_other():
+    from stacr_b200.ops import nn_ops
+    from stacr_b200.optim import clip_grad_norm_
+
+    inv, _ = nn_ops.rotary_frequencies(64, device="cuda")
+    jobs = []
+    for seed, (m, k, f) in enumerate(((700, 512, 1096), (40, 1024, 2056))):
+        x, wg, wu, _, _, dh = gated_inputs(m, k, f, seed=seed)
+        leaves = [t.requires_grad_() for t in (x, wg, wu)]
+        q = torch.randn(2, 33, 4, 64, device="cuda")
+        params = clip_params([(257, 129), (5000,)], (torch.float32,), seed=seed)
+        fresh = [p.grad.clone() for p in params]
+
+        def job(leaves=leaves, dh=dh, q=q, params=params, fresh=fresh):
+            for p, g in zip(params, fresh):
+                p.grad.copy_(g)
+            h = nn_ops.gated_linear(*leaves)
+            grads = torch.autograd.grad(h, leaves, dh)
+            return [h.detach(), *grads, nn_ops.gated_product(q, q + 1), nn_ops.rotary(q, None, inv, 5)[0], clip_grad_norm_(params, 0.3), *(p.grad for p in params)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in job()]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = job()
+        jobs.append((graph, got, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, _, _, stream in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, got, want, _ in jobs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 # ------------------------------------------------------------------------------------------------ gradient norm and clipping
