@@ -685,8 +685,11 @@ def _bf16_operand(weight):
 
 def _weight_gradient_buffer(weight, slot):
     """Where a weight's gradient is formed: the lent slot, else a new matrix, fp32 unless the weight itself is bf16."""
-    return slot if slot is not None else torch.empty(weight.shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32,
-                                                     device=weight.device)
+    if slot is not None:
+        return slot
+    if weight.dtype in (torch.bfloat16, torch.float32) and weight.is_contiguous():
+        return torch.empty_like(weight)
+    return weight.new_empty(weight.shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32)
 
 
 class _GatedLinearFn(torch.autograd.Function):
@@ -702,14 +705,14 @@ class _GatedLinearFn(torch.autograd.Function):
             xa = _operand(x2d)
             h, kept = gated.forward(xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), activation,
                                     keep=not recompute)
-        ctx.save_for_backward(xa, gate_weight, up_weight, gate_bias, up_bias, *(kept or ()))
+        ctx.save_for_backward(xa, gate_weight, up_weight, gate_bias, up_bias, kept)
         ctx.activation, ctx.in_dtype = activation, x2d.dtype
         return h
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dh):
-        xa, gate_weight, up_weight, gate_bias, up_bias, *kept = ctx.saved_tensors
+        xa, gate_weight, up_weight, gate_bias, up_bias, kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dbg = dbu = None
         with _lib.on_device(xa):
@@ -720,7 +723,7 @@ class _GatedLinearFn(torch.autograd.Function):
             dwg = _weight_gradient_buffer(gate_weight, gslot) if need[1] else None
             dwu = _weight_gradient_buffer(up_weight, uslot) if need[2] else None
             d, dx = gated.backward(dh, xa, _bf16_operand(gate_weight), _bf16_operand(up_weight), _f32_bias(gate_bias), _f32_bias(up_bias), ctx.activation,
-                                   kept or None, need[0], dwg, dwu)
+                                   kept, need[0], dwg, dwu)
             if dx is not None and dx.dtype != ctx.in_dtype:
                 dx = dx.to(ctx.in_dtype)
             if dwg is not None:

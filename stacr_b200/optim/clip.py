@@ -51,13 +51,13 @@ def _run(grads, table, max_norm: float | None) -> torch.Tensor:
     from ..ops import _lib
 
     ptrs, sizes, codes = table
-    n, device = len(ptrs), grads[0].device
+    n = len(ptrs)
     if not n:
-        return torch.zeros((), dtype=torch.float32, device=device)
+        return torch.zeros((), dtype=torch.float32, device=grads[0].device)
     with _lib.on_device(grads[0]):
         sms, stream = _lib.place(grads[0])
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        partial = torch.empty(_lib.entry("sb_clip_partials", "ii")(n, sms), dtype=torch.float64, device=device)
+        norm = grads[0].new_empty((), dtype=torch.float32)
+        partial = norm.new_empty(_lib.entry("sb_clip_partials", "ii")(n, sms), dtype=torch.float64)
         ptrs, sizes, codes = array("Q", ptrs), array("q", sizes), array("B", codes)
         rc = _lib.entry("sb_grad_clip", "pppippdiip")(ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], n, partial.data_ptr(), norm.data_ptr(),
                                                      0.0 if max_norm is None else max_norm, max_norm is not None, sms, stream)
