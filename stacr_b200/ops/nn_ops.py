@@ -501,6 +501,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict | None = N
         stretched = float(base) * factor ** (dim / (dim - 2)) if dim > 2 else float(base)
         return stretched ** -index, 1.0
     if kind == "yarn":
+        if base <= 1:
+            raise ValueError(f"rotary scaling 'yarn' needs a base above 1, got {base}")
+
         def pair_with(turns):       # the (real) pair index whose frequency makes this many turns over the original length
             return dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
@@ -537,7 +540,11 @@ class _RotaryFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.first, ctx.interleaved, ctx.scale = first, interleaved, scale
         with _lib.on_device(q):
-            return nn_kernels.rotary(_heads(q), _heads(k), inv_freq, positions, first, interleaved, scale, 1.0)
+            out = nn_kernels.rotary(_heads(q), _heads(k), inv_freq, positions, first, interleaved, scale, 1.0)
+        frozen = [t for t, needed in zip(out, ctx.needs_input_grad) if t is not None and not needed]
+        if frozen:
+            ctx.mark_non_differentiable(*frozen)
+        return out
 
     @staticmethod
     @_differentiable_once
@@ -559,10 +566,10 @@ def rotary(q, k, inv_freq, positions=None, *, interleaved: bool = False, scale: 
     """Rotary positions: ``(q', k')`` for ``q`` ``[B, S, heads, D]`` and ``k`` ``[B, S, kv_heads, D]`` (or ``None``).
 
     ``inv_freq`` (see :func:`rotary_frequencies`) has ``rot / 2`` angular frequencies; the first ``rot <= D`` values of a head are
-    turned (``inv_freq`` itself receives no gradient), as pairs ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)``, and the rest is copied.  Pair ``i`` at position ``p`` is
-    turned by ``p * inv_freq[i]`` and multiplied by ``scale``; the angle is formed in 64 bits.  ``positions`` is ``None`` (``0 .. S-1``),
-    an int (the first token's position), or an integer tensor ``[S]``, ``[1, S]``, ``[B, 1]`` or ``[B, S]``.  Inputs may have any strides
-    (a transposed ``[B, heads, S, D]`` view is read in place); results are contiguous.
+    turned, as pairs ``(i, i + rot / 2)`` or, interleaved, ``(2 i, 2 i + 1)``, and the rest is copied.  Pair ``i`` at position ``p`` is
+    turned by ``p * inv_freq[i]`` and multiplied by ``scale``; the angle is formed in 64 bits, and ``inv_freq`` receives no gradient.
+    ``positions`` is ``None`` (``0 .. S-1``), an int (the first token's position), or an integer tensor ``[S]``, ``[1, S]``, ``[B, 1]``
+    or ``[B, S]``.  Inputs may have any strides (a transposed ``[B, heads, S, D]`` view is read in place); results are contiguous.
     """
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("rotary expects q and k as [batch, sequence, heads, head_dim]")

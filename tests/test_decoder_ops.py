@@ -106,6 +106,7 @@ def test_rotary_frequency_scalings():
 @pytest.mark.parametrize("dim,base,scaling", [
     (7, 1e4, None), (0, 1e4, None), (8, -1.0, None), (8, 1e4, {"rope_type": "spiral", "factor": 2}), (8, 1e4, {"type": "linear"}),
     (8, 1e4, {"type": "linear", "factor": 0.5}), (8, 1e4, {"type": "yarn", "factor": 2}),
+    (8, 1.0, {"type": "yarn", "factor": 2, "original_max_position_embeddings": 64}),
     (8, 1e4, {"type": "llama3", "factor": 2, "original_max_position_embeddings": 64, "low_freq_factor": 4, "high_freq_factor": 4})])
 def test_rotary_frequency_refusals(dim, base, scaling):
     with pytest.raises(ValueError):

@@ -105,6 +105,8 @@ def test_rotary_positions_types_offsets_and_partial_gradients():
     (dk,) = torch.autograd.grad(nn_ops.rotary(q, k, inv)[1].sum(), k)
     (dq,) = torch.autograd.grad(nn_ops.rotary(q, k.detach(), inv)[0].sum(), q)
     assert torch.isfinite(dk).all() and torch.isfinite(dq).all()
+    out = nn_ops.rotary(q.detach(), k, inv)
+    assert not out[0].requires_grad and out[1].requires_grad
     with pytest.raises(RuntimeError):
         (g,) = torch.autograd.grad(nn_ops.rotary(q, None, inv)[0].sum(), q, create_graph=True)
         g.sum().backward()
