@@ -4,8 +4,8 @@
 // The operands change places: 64 rows of Wg and the same 64 of Wu are the 128 rows (tensor memory lanes) of a tcgen05.mma, the
 // tokens, padded to N = 16, 32, 64 or 128, its columns.  So a CTA streams 64 features' weights once, 16 KB a k-block, and no row
 // of the tensor memory is spent on tokens that are not there.  Where there are more CTAs than SMs two share one, with 110 KB of
-// stages each, so that all F / 64 CTAs of a usual width are resident at once.  64 tokens, K 4096, F 14336 (235 MB): 43.4 us, 5.4
-// TB/s or 0.83 of a copy's rate, against 54 for the 256-token tiles; K 2048, F 8192: 15.8 against 19.4.
+// stages each, so that all F / 64 CTAs of a usual width are resident at once.  64 tokens, K 4096, F 14336 (235 MB): 42.3 us, 5.6
+// TB/s or 0.85 of a copy's rate, against 54 for the 256-token tiles; K 2048, F 8192: 15.5 against 19.4.
 // Lanes 0..63 end up with gate, 64..127 with up: the halves trade the tokens they do not finish through shared memory, gate lanes
 // finish the first half of the tokens, up lanes the second.
 #include "gated.cuh"
@@ -56,6 +56,13 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int f0 = blockIdx.x * FT, num_kb = (a.K + BK - 1) / BK;
 
+  auto load = [&](int kb, int s) {
+    uint8_t* at = smem + s * L::STAGE;
+    mbar_expect_tx(&full_bar[s], L::STAGE);
+    tma_load_2d(at, &map_g, &full_bar[s], kb * BK, f0);
+    tma_load_2d(at + W_BYTES / 2, &map_u, &full_bar[s], kb * BK, f0);
+    tma_load_2d(at + W_BYTES, &map_x, &full_bar[s], kb * BK, 0);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -64,6 +71,9 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
+    fence_proxy_async();
+    // the producer has its barriers: the first stages are under way while the others wait for the tensor memory
+    for (int kb = 0; kb < L::STAGES && kb < num_kb; ++kb) load(kb, kb);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, L::COLS);
@@ -77,14 +87,10 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
   if (warp == 0) {
     if (lane == 0) {
       int s = 0;
-      uint32_t ph = 0;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, a.status, ST_TIMEOUT_SMEM_EMPTY)) break;
-        uint8_t* at = smem + s * L::STAGE;
-        mbar_expect_tx(&full_bar[s], L::STAGE);
-        tma_load_2d(at, &map_g, &full_bar[s], kb * BK, f0);
-        tma_load_2d(at + W_BYTES / 2, &map_u, &full_bar[s], kb * BK, f0);
-        tma_load_2d(at + W_BYTES, &map_x, &full_bar[s], kb * BK, 0);
+      uint32_t ph = 0;                                  // parity of the phase in which a stage's first contents are released
+      for (int kb = L::STAGES; kb < num_kb; ++kb) {
+        if (!mbar_wait(&empty_bar[s], ph, abort_flag, a.status, ST_TIMEOUT_SMEM_EMPTY)) break;
+        load(kb, s);
         if (++s == L::STAGES) {
           s = 0;
           ph ^= 1u;

@@ -661,7 +661,7 @@ namespace gg {
 //   gated_tokens.cu (to 64 tokens): 2 us and the weights at 6, 4.9, 3.2 and 1.7 TB/s for 8, 16, 32 and 64 tokens.  Measured at
 //     67 MB (K 2048, F 8192): 12.5, 15.3, 20.6, 40.8 us, at 4 MB (K 512, F 2048): 2.3, 2.7, 3.3, 4.7.
 //   gated_few.cu: 4.4 us and 0.27 for each k-block, or 3.5 and the weights at 5.9 TB/s, and more for more columns to finish.
-//     Measured at the same: 15.1, 15.4, 15.9, 15.8 us (128 tokens: 17.9); 5.9, 5.9, 6.0, 6.7 (8.3).
+//     Measured at the same: 15.2 us to 32 tokens, 15.5, and 17.0 for 128; 5.9 to 32 tokens, 6.7, 8.5.
 //   tiles, 128 tokens: 19.8 and 9.3.
 static bool streams_fragments(int M, int K, int F) {
   if (M > 64) return false;
