@@ -7,7 +7,9 @@
 // kernel's parameters: no copy to the device, and a captured call keeps its own.
 //
 // Bound by memory: N values read, and when the norm is above the bound N read and written again.  The second kernel takes its
-// chunks from the last to the first, since the end of what the first one read is what L2 still holds.
+// chunks from the last to the first, since the end of what the first one read is what L2 still holds.  2^30 fp32 values: norm 610 us
+// (7.0 TB/s), with scaling 2038 (three passes at 0.97 of a copy's rate); bf16 305 and 1040.  Chunks of 4 K to 64 K values, four CTAs
+// an SM and streaming stores all measured within 2 %.
 //
 // Sums: 16 squares in fp32, those sums in fp64.  Sixteen squares that leave fp32's range (|g| beyond 1e19 or below 1e-15) are
 // redone in fp64.

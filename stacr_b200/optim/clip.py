@@ -80,7 +80,7 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
                     error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """Scale all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and return their norm from before, as a device scalar.
 
-    The call of ``torch.nn.utils.clip_grad_norm_``.  Dense bf16, fp16 and fp32 gradients on one GPU take the kernels, which sum the
+    Dense bf16, fp16 and fp32 gradients on one GPU take the kernels, which sum the
     2-norm beyond fp32's range and decide about the scaling on the device, so the host does not wait (``error_if_nonfinite``
     does, and raises before anything is scaled) and the call can be captured into a CUDA graph.  A gradient that occurs
     twice counts and is scaled once; gradients that overlap in part are refused.  Everything else (other norms, other layouts or
