@@ -50,7 +50,8 @@ def is_plain_linear(module: nn.Module) -> bool:
     """Whether calling ``module`` computes ``nn_ops.linear`` of its weight and bias and nothing else, so that its operands may be used
     directly: not a wrapped, compressed, adapted or hooked layer."""
     return (type(module) is Linear and "forward" not in module.__dict__ and not (
-        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+        or nn.modules.module._has_any_global_hook()))
 
 
 def saved_tensors_are_hooked() -> bool:

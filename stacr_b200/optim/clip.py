@@ -80,11 +80,11 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
                     error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """Scale all gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and return their norm from before, as a device scalar.
 
-    Dense bf16, fp16 and fp32 gradients on one GPU take the kernels, which sum the
-    2-norm beyond fp32's range and decide about the scaling on the device, so the host does not wait (``error_if_nonfinite``
-    does, and raises before anything is scaled) and the call can be captured into a CUDA graph.  A gradient that occurs
-    twice counts and is scaled once; gradients that overlap in part are refused.  Everything else (other norms, other layouts or
-    devices, sharded tensors) goes to the framework's function, with ``foreach``.
+    Dense bf16, fp16 and fp32 gradients on one GPU take the kernels, which sum the 2-norm beyond fp32's range and decide about the
+    scaling on the device, so the host does not wait (``error_if_nonfinite`` does, and raises before anything is scaled) and the
+    call can be captured into a CUDA graph.  A gradient that occurs twice counts and is scaled once; gradients that overlap in part
+    are refused.  Everything else (other norms, other layouts or devices, sharded tensors) goes to the framework's function, with
+    ``foreach``.
     """
     max_norm, norm_type = float(max_norm), float(norm_type)
     params = _parameters(parameters)
@@ -95,8 +95,7 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
     if error_if_nonfinite:
         norm = _run(grads, table, None)
         if not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped. "
-                               "To disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+            raise RuntimeError(f"the gradients' norm is {float(norm)}: they were left unscaled (error_if_nonfinite)")
     norm = _run(grads, table, max_norm)
     torch.autograd.graph.increment_version(grads)
     return norm

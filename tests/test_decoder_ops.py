@@ -170,5 +170,9 @@ def test_is_plain_linear_sees_wrapped_and_hooked_layers():
     assert not is_plain_linear(layer)
     handle.remove()
     assert is_plain_linear(layer)
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *_: None)
+    assert not is_plain_linear(layer)
+    handle.remove()
+    assert is_plain_linear(layer)
     layer.forward = lambda x: x
     assert not is_plain_linear(layer)
