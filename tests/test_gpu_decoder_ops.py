@@ -672,6 +672,37 @@ def test_llama_under_saved_tensor_hooks_saves_what_separate_layers_save():
     assert sum(t.dtype == torch.bfloat16 and t.shape[-1] == 688 and t.numel() == 40 * 688 for t in saved) >= 8
 
 
+def test_llama_mlp_with_compressed_projections_runs_the_gated_product():
+    import stacr_b200 as S
+    from stacr_b200.models import build_model
+    from stacr_b200.ops import nn_kernels
+
+    torch.manual_seed(0)
+    model = build_model("llama-tiny").cuda()
+    layers = S.apply_stacr(model, rank=8, residual_budget=0.01, surface="mlp", min_features=64)
+    S.set_step(layers, 0)
+    mlp = model.model.layers[0].mlp
+    x = torch.randn(2, 64, 256, device="cuda").bfloat16()          # the basis kernels take multiples of 8 rows
+    calls = []
+    real = nn_kernels.gated_product_fwd
+    nn_kernels.gated_product_fwd = lambda *a: calls.append(1) or real(*a)
+    try:
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = mlp(x)
+            assert len(calls) == 1
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+                z = mlp(x)                     # the activation and the product as two ops
+            assert len(calls) == 1
+            gate, up = mlp.gate_proj(x).double(), mlp.up_proj(x).double()
+    finally:
+        nn_kernels.gated_product_fwd = real
+    # h is rounded once here and twice there, so the two differ by three half steps of it at most, each output by one more
+    h, w, e = (F.silu(gate) * up).abs().detach(), mlp.down_proj.weight.detach().to(torch.bfloat16).double().abs(), HALF[torch.bfloat16]
+    inside(y.detach(), z.detach().double(), 3 * e * (1 + e) * (h @ w.t()) + 2 * e * z.detach().double().abs() + 1e-6)
+    y.float().square().mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in mlp.parameters() if p.grad is not None)
+
+
 def test_llama_step_replayed_from_a_cuda_graph_equals_the_eager_step():
     from stacr_b200.models import build_model
     from stacr_b200.optim import clip_grad_norm_
