@@ -72,9 +72,14 @@ __device__ __forceinline__ float exp_f32(float x) {
 
 // 1 / (1 + e^-x).  e^-x overflows to infinity below x = -88, where the result is 0.  FAST: the hardware's exponential and reciprocal,
 // off by (3 + 1.2 |x|) 2^-23 of the result: for results that are rounded to 16-bit types (fp16: 2^-11) or kept in 24 bits (2^-16).
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_f32(float x) {
-  return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : __frcp_rn(1.f + exp_f32(-x));
+  return FAST ? rcp_fast(1.f + __expf(-x)) : __frcp_rn(1.f + exp_f32(-x));
 }
 
 // act(x) and act'(x):
@@ -86,7 +91,7 @@ __device__ __forceinline__ void act_and_derivative(float x, float& act, float& d
   if (ACT == ACT_GELU && FAST) {
     // Abramowitz and Stegun 7.1.26, erfc(z) = (a1 t + ... + a5 t^5) e^-z^2 with t = 1 / (1 + p z), off by at most 1.5e-7; the
     // exponential is the density's too (8192 x 8192 values in bf16: 76 us forward and 114 backward, 93 and 131 with erff)
-    const float e = __expf(-0.5f * x * x), t = __fdividef(1.f, fmaf(0.3275911f * 0.707106781f, fabsf(x), 1.f));
+    const float e = __expf(-0.5f * x * x), t = rcp_fast(fmaf(0.3275911f * 0.707106781f, fabsf(x), 1.f));
     const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
     const float cdf = x < 0.f ? tail : 1.f - tail;
     act = x * cdf;
@@ -102,12 +107,6 @@ __device__ __forceinline__ void act_and_derivative(float x, float& act, float& d
     act = x * s;
     der = s * fmaf(x * (1.f - s), slope, 1.f);
   }
-}
-
-// Upper 24 bits of a float, rounded; NaN and infinity keep theirs.
-__device__ __forceinline__ unsigned upper24(float v) {
-  const unsigned b = __float_as_uint(v);
-  return (b & 0x7fffffffu) < 0x7f800000u ? b + 0x80u : b;
 }
 
 template <int ACT, bool FAST>

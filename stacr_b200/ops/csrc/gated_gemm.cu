@@ -11,7 +11,8 @@
 // main loop nothing: per k-block and CTA the same 32 KB as a plain 256 x 256 GEMM tile.
 //
 // What backward needs of G and U are two factors, dG = dh A and dU = dh B with A = U act'(G), B = act(G).  When they are kept, the
-// forward epilogue writes each as the upper 24 bits of its fp32 value, 16 in one matrix and 8 in another: kept in bf16 they
+// forward epilogue writes each as the upper 24 bits of its fp32 value (cut, off by at most 2^-15; rounding them took as many
+// instructions as forming them), 16 in one matrix and 8 in another: kept in bf16 they
 // would add as much error to the weight gradients as the bf16 rounding of dG itself does (relative error 3.0e-3 against 2.3e-3),
 // and the three bytes are the two factors' share of what separate layers keep (gate, act(gate), up in bf16: six bytes a feature).
 //
@@ -100,15 +101,15 @@ __device__ __forceinline__ void put16(uint8_t* base, int row, int unit, const fl
   *stage2(base, row, unit) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
   *stage2(base, row, unit + 1) = make_uint4(pack_bf16x2(f[8], f[9]), pack_bf16x2(f[10], f[11]), pack_bf16x2(f[12], f[13]), pack_bf16x2(f[14], f[15]));
 }
-// 16 values as their upper 16 and next 8 bits
+// 16 values as their upper 16 and next 8 bits; the last 8 are cut off (a NaN that arithmetic made keeps bits above them)
 __device__ __forceinline__ void put24(uint8_t* hi, uint8_t* lo, int row, int unit, const float (&f)[16]) {
   uint32_t h[8], l[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = __byte_perm(upper24(f[2 * i]), upper24(f[2 * i + 1]), 0x7632);
+  for (int i = 0; i < 8; ++i) h[i] = __byte_perm(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]), 0x7632);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t p = __byte_perm(upper24(f[4 * i]), upper24(f[4 * i + 1]), 0x0051);
-    const uint32_t q = __byte_perm(upper24(f[4 * i + 2]), upper24(f[4 * i + 3]), 0x0051);
+    const uint32_t p = __byte_perm(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), 0x0051);
+    const uint32_t q = __byte_perm(__float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]), 0x0051);
     l[i] = __byte_perm(p, q, 0x5410);
   }
   *stage2(hi, row, unit) = make_uint4(h[0], h[1], h[2], h[3]);

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 8 ? 1 : 2) gated_tokens_kern
     const size_t at = static_cast<size_t>(m) * a.F + f;
     a.h[at] = __float2bfloat16_rn(act * up);
     if (a.a_hi) {
-      const unsigned fa = upper24(up * der), fb = upper24(act);
+      const unsigned fa = __float_as_uint(up * der), fb = __float_as_uint(act);
       a.a_hi[at] = static_cast<unsigned short>(fa >> 16);
       a.b_hi[at] = static_cast<unsigned short>(fb >> 16);
       a.a_lo[m * a.ld_lo + f] = static_cast<unsigned char>(fa >> 8);

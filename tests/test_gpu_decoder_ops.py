@@ -219,7 +219,7 @@ def gated_bounds(x, wg, wu, bg, bu, dh, act, g, u, keep):
     """Bounds of (h, dx, dWg, dWu, dbg, dbu), element by element.
 
     A projection is off by its fp32 summation, at most (K + 2) 2^-24 times the sum of its terms' sizes; |act'| <= 1.13, |act''| <= 1.
-    The factors that are kept for backward have 24 bits (half a step: 2^-16).  The derivative's products are rounded to bf16 before they are
+    The factors that are kept for backward are cut to 24 bits (one step: 2^-15).  The derivative's products are rounded to bf16 before they are
     multiplied again; sums over F or the tokens in fp32 add their length times 2^-24; every result is rounded once.
     """
     e, f32 = HALF[torch.bfloat16], 2.0 ** -24
@@ -235,7 +235,7 @@ def gated_bounds(x, wg, wu, bg, bu, dh, act, g, u, keep):
     fp = 16 * f32 * g.abs().clamp_min(1.2)
     bh = (a * U) * e + (1.13 * eg + fp) * (U + eu) + a * eu + 1e-30
     ea, eda = 1.13 * eg + fp, eg + fp
-    kept = 2.0 ** -16 if keep else 0.0
+    kept = 2.0 ** -15 if keep else 0.0
     edg = D * ((eda * (U + eu)) + da * eu + kept * (U + eu) * (da + eda))
     edu = D * (ea + kept * (a + ea))
     DG, DU = D * U * da, D * a
