@@ -161,6 +161,64 @@ def test_llama_scaled_positions_change_the_model_and_default_ones_do_not():
     torch.testing.assert_close(a, c, rtol=1e-4, atol=1e-4)
 
 
+# ---- csrc/gated_gemm.cu restated on the host: how reductions are shared among CTA pairs, and in which order tiles are taken
+def shares(tiles, num_kb, sms):
+    pairs = max(1, sms // 2)
+    last = tiles % pairs
+    if last == 0:
+        return tiles, 1
+    splits = min(pairs // last, num_kb // 8)
+    if splits < 2:
+        return tiles, 1
+    per = -(-num_kb // splits)
+    splits = -(-num_kb // per)
+    return (tiles, 1) if num_kb - per < 24 else (tiles - last, splits)
+
+
+@pytest.mark.parametrize("sms", [148, 132, 5, 2, 1])
+def test_split_reductions_cover_every_block_once_and_fit_one_round(sms):
+    for tiles in (1, 2, 7, 16, 37, 73, 74, 75, 256, 300, 1792):
+        for num_kb in (1, 2, 8, 23, 32, 33, 64, 127, 256, 449):
+            whole, splits = shares(tiles, num_kb, sms)
+            pairs, per, covered = max(1, sms // 2), -(-num_kb // splits), {}
+            parts = 0
+            for u in range(whole + (tiles - whole) * splits):
+                if u < whole:
+                    tile, lo, hi = u, 0, num_kb
+                else:
+                    v = u - whole
+                    tile, k = whole + v // splits, v % splits
+                    lo, hi = k * per, min((k + 1) * per, num_kb)
+                    assert v == parts
+                    parts += 1
+                assert lo < hi, "a part without blocks would leave its sums unwritten"
+                covered.setdefault(tile, []).extend(range(lo, hi))
+            assert all(covered[t] == list(range(num_kb)) for t in range(tiles)) and len(covered) == tiles
+            assert parts <= pairs and (whole % pairs == 0 or whole == tiles)
+
+
+@pytest.mark.parametrize("rows", [4, 16])
+def test_tile_order_visits_every_tile_once(rows):
+    for num_m, num_n in ((1, 1), (3, 7), (4, 5), (17, 3), (32, 64), (33, 2)):
+        seen = set()
+        for tile in range(num_m * num_n):
+            first = tile // (rows * num_n) * rows
+            height, r = min(rows, num_m - first), tile % (rows * num_n)
+            seen.add((first + r % height, r // height))
+        assert seen == {(m, n) for m in range(num_m) for n in range(num_n)}
+
+
+def test_factors_cut_to_24_bits_join_to_the_value_within_a_step():
+    v = torch.cat((torch.randn(4096), torch.tensor([0.0, -0.0, 1e-38, 3e38, float("inf"), -float("inf")])))
+    bits = v.view(torch.int32)
+    hi, lo = (bits >> 16) & 0xffff, (bits >> 8) & 0xff
+    joined = ((hi << 16) | (lo << 8)).to(torch.int32).view(torch.float32)
+    finite = torch.isfinite(v)
+    assert torch.equal(joined[~finite], v[~finite])
+    assert bool(((joined - v).abs()[finite] <= v.abs()[finite] * 2.0 ** -15).all())
+    assert bool(torch.tensor([0x7fffff00], dtype=torch.int32).view(torch.float32).isnan())      # what arithmetic's NaN is cut to
+
+
 def test_is_plain_linear_sees_wrapped_and_hooked_layers():
     from stacr_b200.models.common import Linear, is_plain_linear
 
