@@ -53,6 +53,7 @@ struct GatedItem {
 
 template <typename T, int VEC, int ACT, bool BWD>
 __global__ void __launch_bounds__(256) gated_product_kernel(const GatedArgs a) {
+  after_predecessors();
   const long long nv = a.n / VEC, step = static_cast<long long>(gridDim.x) * blockDim.x;
   for (long long r = blockIdx.y * static_cast<long long>(blockDim.y) + threadIdx.y; r < a.rows; r += static_cast<long long>(gridDim.y) * blockDim.y) {
     const T* gate = static_cast<const T*>(a.gate) + r * a.ld_gate;
@@ -89,10 +90,9 @@ static int gated_launch(const GatedArgs& a, int act, int sms, cudaStream_t st) {
   if (by > cap) by = cap;
   if (by > 65535) by = 65535;
   const dim3 grid(gx, static_cast<unsigned>(by));
-  if (act == ACT_SILU) gated_product_kernel<T, VEC, ACT_SILU, BWD><<<grid, block, 0, st>>>(a);
-  else if (act == ACT_GELU) gated_product_kernel<T, VEC, ACT_GELU, BWD><<<grid, block, 0, st>>>(a);
-  else gated_product_kernel<T, VEC, ACT_GELU_TANH, BWD><<<grid, block, 0, st>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  if (act == ACT_SILU) return launch_early(gated_product_kernel<T, VEC, ACT_SILU, BWD>, grid, block, 0, st, a);
+  if (act == ACT_GELU) return launch_early(gated_product_kernel<T, VEC, ACT_GELU, BWD>, grid, block, 0, st, a);
+  return launch_early(gated_product_kernel<T, VEC, ACT_GELU_TANH, BWD>, grid, block, 0, st, a);
 }
 
 // The widest power-of-two vector (in elements) that every operand's address and row stride allow, at most 16 bytes.  Of one row, the

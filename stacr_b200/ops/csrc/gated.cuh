@@ -23,6 +23,28 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Launches that may begin while the kernel before them in the stream drains: the launch itself and what a kernel does before
+// after_predecessors() (barriers, tensor memory) are then hidden.  A launch made this way starts when every block of its
+// predecessor has ended, but nothing else orders it behind that kernel's stores: so every thread calls after_predecessors(), which
+// waits for the predecessor's completion, before its first access to global memory.  33 tokens of K 1536, F 8960, one call after
+// another: 16.3 us without, 13.4 with; one token of K 2048, F 8192: 13.7 and 11.9.
+__device__ __forceinline__ void after_predecessors() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+static int launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+}
+
 // VEC neighbouring values as one access, and to and from fp32 (16-bit types two at a time).
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {

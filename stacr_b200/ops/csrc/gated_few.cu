@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
+    after_predecessors();
     // the producer has its barriers: the first stages are under way while the others wait for the tensor memory
     for (int kb = 0; kb < L::STAGES && kb < num_kb; ++kb) load(kb, kb);
   }
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(THREADS) gated_few_kernel(const __grid_constan
     tmem_alloc(tmem_slot, L::COLS);
     tmem_relinquish();
   }
+  after_predecessors();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -215,8 +217,7 @@ static int launch(const void* x, const void* wg, const void* wu, const Args& a, 
   if (!rc) rc = make_tensor_map_bf16(&mu, wu, a.K, a.F, a.K, FT);
   if (!rc) rc = make_tensor_map_bf16(&mx, x, a.K, a.M, a.K, N);
   if (rc) return rc;
-  gated_few_kernel<N, ALONE, ACT><<<(a.F + FT - 1) / FT, THREADS, L::BYTES, st>>>(mg, mu, mx, a);
-  return static_cast<int>(cudaGetLastError());
+  return launch_early(gated_few_kernel<N, ALONE, ACT>, dim3((a.F + FT - 1) / FT), dim3(THREADS), L::BYTES, st, mg, mu, mx, a);
 }
 
 template <bool ALONE, int ACT>

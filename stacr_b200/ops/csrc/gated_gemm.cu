@@ -235,6 +235,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
     tmem_alloc_pair(tmem_slot, TMEM_COLS);
     tmem_relinquish_pair();
   }
+  after_predecessors();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -450,6 +451,7 @@ gated_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_cons
 // Sums of the parts of the split tiles, in the order of the parts.  A block has 16 columns of a tile, a thread one row of them.
 template <int MODE>
 __global__ void __launch_bounds__(TM) gated_join_kernel(const __grid_constant__ Params p) {
+  after_predecessors();
   const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + TN - 1) / TN, tiles_one = num_m * num_n;
   const int split_tile = blockIdx.x >> 4, c = blockIdx.x & 15;
   const int tile = p.whole + split_tile, problem = MODE == WEIGHT_GRAD && tile >= tiles_one ? 1 : 0;
@@ -530,19 +532,20 @@ static int launch(const CUtensorMap& a0, const CUtensorMap& a1, const CUtensorMa
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // see launch_early
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a0, a1, b0, b1, p);
   if (e != cudaSuccess) return static_cast<int>(e);
   if constexpr (MODE == INPUT_GRAD || MODE == WEIGHT_GRAD) {
     if (tiles > p.whole) {
-      gated_join_kernel<MODE><<<static_cast<unsigned>((tiles - p.whole) * 16), TM, 0, stream>>>(p);
-      return static_cast<int>(cudaGetLastError());
+      return launch_early(gated_join_kernel<MODE>, dim3(static_cast<unsigned>((tiles - p.whole) * 16)), dim3(TM), 0, stream, p);
     }
   }
   return 0;
@@ -566,6 +569,7 @@ __device__ __forceinline__ float join24(unsigned hi, unsigned lo) { return __uin
 __global__ void __launch_bounds__(256) gated_factors_kernel(const uint4* __restrict__ dh, const uint4* __restrict__ a_hi, const unsigned char* __restrict__ a_lo,
                                                             const uint4* __restrict__ b_hi, const unsigned char* __restrict__ b_lo, uint4* __restrict__ dg,
                                                             uint4* __restrict__ du, int rows, int nv, long long ld_lo) {
+  after_predecessors();
   for (int r = blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += gridDim.y * blockDim.y)
     for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < nv; c += gridDim.x * blockDim.x) {
       const size_t i = static_cast<size_t>(r) * nv + c;
@@ -618,9 +622,8 @@ static int factors(const void* dh, const unsigned short* hi, const unsigned char
   const long long cap = (sms * 32ll + gx - 1) / gx, by = (M + static_cast<int>(block.y) - 1) / static_cast<int>(block.y);
   const long long lim = cap < 65535 ? cap : 65535;
   const dim3 grid(gx, static_cast<unsigned>(by < lim ? by : lim));
-  gated_factors_kernel<<<grid, block, 0, st>>>(static_cast<const uint4*>(dh), reinterpret_cast<const uint4*>(hi), lo, reinterpret_cast<const uint4*>(hi + mf),
-                                               lo + M * ld_lo, reinterpret_cast<uint4*>(d), reinterpret_cast<uint4*>(d + mf), M, nv, ld_lo);
-  return static_cast<int>(cudaGetLastError());
+  return launch_early(gated_factors_kernel, grid, block, 0, st, static_cast<const uint4*>(dh), reinterpret_cast<const uint4*>(hi), lo,
+                      reinterpret_cast<const uint4*>(hi + mf), lo + M * ld_lo, reinterpret_cast<uint4*>(d), reinterpret_cast<uint4*>(d + mf), M, nv, ld_lo);
 }
 
 // dx[M, K] = dG Wg + dU Wu

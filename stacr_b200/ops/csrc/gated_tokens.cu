@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 8 ? 1 : 2) gated_tokens_kern
                                a.wu + static_cast<size_t>(r1) * a.K};
   float cg[NT][4] = {}, cu[NT][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
+  after_predecessors();
   for (int k0 = warp * KB; k0 < a.K; k0 += WARPS * KB * U) {
     uint4 v[U][4], bx[U][NT];
 #pragma unroll
@@ -126,8 +127,7 @@ static int launch(const Args& a, cudaStream_t st) {
     if (e != cudaSuccess) return static_cast<int>(e);
     *configured = true;
   }
-  gated_tokens_kernel<NT, U, ACT><<<(a.F + FT - 1) / FT, WARPS * 32, bytes, st>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  return launch_early(gated_tokens_kernel<NT, U, ACT>, dim3((a.F + FT - 1) / FT), dim3(WARPS * 32), bytes, st, a);
 }
 
 template <int ACT>

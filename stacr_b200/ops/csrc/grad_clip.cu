@@ -128,6 +128,7 @@ __device__ __forceinline__ int locate(const ClipTable& t, int c, long long& star
 __global__ void __launch_bounds__(CLIP_THREADS) grad_squares_kernel(const __grid_constant__ ClipTable t, double* __restrict__ partial) {
   __shared__ double red[CLIP_THREADS / 32];
   double acc = 0.0;
+  after_predecessors();
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     long long start, len;
     const int i = locate(t, c, start, len);
@@ -144,6 +145,7 @@ __global__ void __launch_bounds__(CLIP_THREADS) grad_scale_kernel(const __grid_c
                                                                   double max_norm, int scale, float* __restrict__ norm_out) {
   __shared__ double red[CLIP_THREADS / 32];
   double acc = 0.0;
+  after_predecessors();
   for (int i = threadIdx.x; i < n_partial; i += CLIP_THREADS) acc += partial[i];
   const double norm = sqrt(block_sum(acc, red));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(norm);
@@ -209,9 +211,8 @@ extern "C" int sb_grad_clip(void* const* ptrs, const long long* numel, const uns
     const int m = n - lo < CLIP_TENSORS ? n - lo : CLIP_TENSORS;
     if (!fill_table(t, ptrs + lo, numel + lo, dtype + lo, m, chunk)) return -2;
     const int grid = t.chunks < ctas ? t.chunks : ctas;
-    grad_squares_kernel<<<grid, CLIP_THREADS, 0, st>>>(t, partial + parts);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return static_cast<int>(e);
+    const int rc = launch_early(grad_squares_kernel, dim3(grid), dim3(CLIP_THREADS), 0, st, t, partial + parts);
+    if (rc) return rc;
     parts += grid;
   }
   // the groups in reverse: the last one's table is still in t, and its end is what L2 holds
@@ -219,9 +220,8 @@ extern "C" int sb_grad_clip(void* const* ptrs, const long long* numel, const uns
     const int m = n - lo < CLIP_TENSORS ? n - lo : CLIP_TENSORS;
     fill_table(t, ptrs + lo, numel + lo, dtype + lo, m, chunk);
     const int grid = !scale ? 1 : t.chunks < ctas ? t.chunks : ctas;
-    grad_scale_kernel<<<grid, CLIP_THREADS, 0, st>>>(t, partial, parts, max_norm, scale, norm_out);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return static_cast<int>(e);
+    const int rc = launch_early(grad_scale_kernel, dim3(grid), dim3(CLIP_THREADS), 0, st, t, partial, parts, max_norm, scale, norm_out);
+    if (rc) return rc;
     if (!scale) break;
   }
   return 0;

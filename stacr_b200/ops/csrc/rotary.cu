@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(VEC == 1 ? 512 : ROT_THREADS, VEC == 1 ? 2 : 4
   const bool isq = h < a.hq, works = h < a.hq + a.hk;
   const long long sstep = isq ? a.qs : a.ks, dstep = static_cast<long long>(isq ? a.hq : a.hk) * a.D;
 
+  after_predecessors();
   for (long long b = blockIdx.y; b < a.B; b += gridDim.y) {
     const T* src = nullptr;
     T* dst = nullptr;
@@ -178,8 +179,7 @@ static int rotary_launch(const RotaryArgs& a, int sms, cudaStream_t st) {
   if (tokens * row > 48 * 1024) tokens = 1;
   const long long by = a.B < 65535 ? a.B : 65535;
   const dim3 grid((a.S + tokens - 1) / tokens, static_cast<unsigned>(by), rounds);
-  rotary_kernel<T, VEC, INTER, MIXED><<<grid, slots * side, tokens * row, st>>>(a, side, tokens);
-  return static_cast<int>(cudaGetLastError());
+  return launch_early(rotary_kernel<T, VEC, INTER, MIXED>, grid, dim3(slots * side), tokens * row, st, a, side, tokens);
 }
 
 // The widest power-of-two vector that divides every extent, stride and address, at most 16 bytes; `parts`: the rotary part too.
