@@ -4,8 +4,8 @@
 // The operands change places: 64 rows of Wg and the same 64 of Wu are the 128 rows (tensor memory lanes) of a tcgen05.mma, the
 // tokens, padded to N = 16, 32, 64 or 128, its columns.  So a CTA streams 64 features' weights once, 16 KB a k-block, and no row
 // of the tensor memory is spent on tokens that are not there.  Where there are more CTAs than SMs two share one, with 110 KB of
-// stages each, so that all F / 64 CTAs of a usual width are resident at once.  64 tokens, K 4096, F 14336 (235 MB): 42.3 us, 5.6
-// TB/s or 0.85 of a copy's rate, against 54 for the 256-token tiles; K 2048, F 8192: 15.5 against 19.4.
+// stages each, so that all F / 64 CTAs of a usual width are resident at once.  64 tokens, K 4096, F 14336 (235 MB): 41.8 us, 5.6
+// TB/s or 0.86 of a copy's rate, against 54 for the 256-token tiles; K 2048, F 8192: 15.0 against 19.3.
 // Lanes 0..63 end up with gate, 64..127 with up: the halves trade the tokens they do not finish through shared memory, gate lanes
 // finish the first half of the tokens, up lanes the second.
 #include "gated.cuh"

@@ -1,6 +1,6 @@
 // Gated projections of single tokens: h[M, F] = act(x Wg^T + bg) * (x Wu^T + bu) for M <= 64 (see sb_gated_forward for when).
 //
-// Bound by the weights, 4 K F bytes that are read once (one token, K 4096, F 14336: 39.8 us, 5.9 TB/s, 0.90 of a copy's rate);
+// Bound by the weights, 4 K F bytes that are read once (one token, K 4096, F 14336: 38.3 us, 6.1 TB/s, 0.94 of a copy's rate);
 // everything here serves that stream.  A CTA owns 16 features (16 rows of
 // each weight) and its eight warps share the reduction: warp w takes every eighth block of 32 values, so that the CTA reads 512
 // contiguous bytes of a row at a time.  Weights go from memory straight into the A fragments of mma.m16n8k16 (features are the
