@@ -360,6 +360,23 @@ def test_gated_linear_uses_lent_gradient_slots():
     assert bool((flat[:32] == 7).all() and (flat[-32:] == 7).all())
 
 
+@pytest.mark.parametrize("recompute", [False, True])
+def test_operators_survive_offloaded_saved_tensors(recompute):
+    from stacr_b200.ops import nn_ops
+
+    x, wg, wu, _, _, dh = gated_inputs(150, 64, 136)
+    inv, _ = nn_ops.rotary_frequencies(64, device="cuda")
+    results = []
+    for offload in (False, True):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, wg, wu)]
+        with torch.autograd.graph.save_on_cpu(pin_memory=True) if offload else torch.enable_grad():
+            h = nn_ops.gated_linear(*leaves, recompute=recompute)
+            p = nn_ops.gated_product(leaves[0], leaves[0])
+            q, _ = nn_ops.rotary(leaves[0].view(10, 15, 1, 64), None, inv, 3)
+        results.append([*torch.autograd.grad(h, leaves, dh), *torch.autograd.grad(p.sum() + q.square().sum(), leaves[0])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("m", [3, 70])
 def test_gated_linear_takes_operands_of_any_alignment_and_order(m):
     from stacr_b200.ops import nn_ops
